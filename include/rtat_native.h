@@ -263,6 +263,124 @@ rtat_status_t rtat_strsm_ex(rtat_handle_t handle, rtat_side_t side, rtat_fill_t 
                             const float* alpha, const float* A, int lda, float* B, int ldb,
                             int variant);
 
+/* ---- products of a trained linear layer ------------------------------------------------
+ * Matrix products on 16-bit operands (f32 accumulation on the matrix cores) with the layer's
+ * elementwise work in the same launch, the gradients of such a product, and the
+ * orthogonalisation of an update to its weight.  No counterpart in the reference.
+ *
+ * Storage is column-major as everywhere in this header.  A framework that stores row-major
+ * activations X (tokens x in), Y (tokens x out) and a weight W (out x in) passes its tensors as
+ * they are: Y^T (out x tokens) = W X^T is transa = T, transb = N, m = out, n = tokens, k = in,
+ * with the row strides as leading dimensions.
+ *
+ * Any m, n, k, leading dimension and element-aligned pointer is accepted; operands whose base
+ * and leading dimension are multiples of 16 bytes are read faster.  An output may not overlap
+ * an input or another output unless a function says so. */
+
+/* Element types.  Numeric values equal hipDataType. */
+typedef enum { RTAT_TYPE_F32 = 0, RTAT_TYPE_F16 = 2, RTAT_TYPE_BF16 = 14 } rtat_type_t;
+
+/* act(z), z in f32:
+ *   RELU       max(z, 0); a NaN stays NaN; derivative 0 at 0
+ *   GELU       z Phi(z), Phi the normal distribution function
+ *   GELU_TANH  z / (1 + exp(-2u)), u = sqrt(2/pi) (z + 0.044715 z^3)
+ *   SILU       z / (1 + exp(-z)) */
+typedef enum {
+  RTAT_ACT_NONE = 0,
+  RTAT_ACT_RELU = 1,
+  RTAT_ACT_GELU = 2,
+  RTAT_ACT_GELU_TANH = 3,
+  RTAT_ACT_SILU = 4,
+  RTAT_ACT_COUNT = 5
+} rtat_activation_t;
+/* "none" / "relu" / "gelu" / "gelu_tanh" / "silu"; NULL when out of range. */
+const char* rtat_activation_name(int act);
+
+/* What rtat_gemm_ep does to a product beside scaling it. */
+typedef struct rtat_epilogue {
+  rtat_activation_t act;
+  const void* bias; /* m values of the operands' type, one per row, or NULL (none) */
+  void* aux;        /* receives the argument of the activation, m x n of the operands' type, or NULL */
+  int ldaux;
+} rtat_epilogue_t;
+
+/* D(m x n) = act(alpha * op(A) * op(B) + bias * 1^T) + beta * C.
+ * A and B are of `type` (F16 or BF16); C (the residual) and D are of `d_type`, which is `type` or
+ * F32.  Sums, bias, activation and residual are formed in f32 and rounded once.  `epilogue` may
+ * be NULL (no activation, bias or aux).  With beta == 0 C is not read and may be NULL; D may be C
+ * (same ldc).  With alpha == 0 or k == 0 A and B are not read.
+ * Long products with few tiles are cut along k into the handle's slice scratch (rtat_create) and
+ * summed in a fixed order; with a lent workspace they are not cut. */
+rtat_status_t rtat_gemm_ep(rtat_handle_t handle, rtat_type_t type, rtat_operation_t transa,
+                           rtat_operation_t transb, int m, int n, int k, const float* alpha,
+                           const void* A, int lda, const void* B, int ldb,
+                           const rtat_epilogue_t* epilogue, const float* beta, const void* C,
+                           int ldc, rtat_type_t d_type, void* D, int ldd);
+
+/* Where rtat_gemm_ep_backward puts its results; a NULL pointer leaves that one out.
+ * dA = alpha * (gradient) + da_beta * dA has A's storage (m x k, or k x m when transa == T), dB
+ * likewise B's; each is of the operands' type or F32.  With a beta of 0 the old values are not
+ * read. */
+typedef struct rtat_gemm_grads {
+  void* dZ; /* m x n of the operands' type: gradient at the activation's argument.  Required when
+               act != NONE and dA or dB is wanted; may be dD itself (lddz == lddd).  Not written
+               when act == NONE: there dZ is dD. */
+  int lddz;
+  rtat_type_t da_type;
+  float da_beta;
+  void* dA;
+  int ldda;
+  rtat_type_t db_type;
+  float db_beta;
+  void* dB;
+  int lddb;
+  float* dbias; /* m row sums of dZ in f32, from the values before dZ is rounded */
+} rtat_gemm_grads_t;
+
+/* The gradients of D = act(alpha * op(A) * op(B) + bias) + beta * C, given dD (m x n) and Z, the
+ * `aux` that the forward call left (not read when act == NONE):
+ *   dZ = dD * act'(Z),  dbias = row sums of dZ,
+ *   d op(A) = alpha * dZ * op(B)^T,  d op(B) = alpha * op(A)^T * dZ   (dC is beta * dD).
+ * The two products read dZ as it is stored, rounded to the operands' type.  dbias takes
+ * rtat_dbias_workspace_bytes(m, n) of the handle's scratch (see rtat_set_workspace: owned and
+ * grown, or lent; RTAT_STATUS_ALLOC_FAILED when it cannot be had). */
+rtat_status_t rtat_gemm_ep_backward(rtat_handle_t handle, rtat_type_t type,
+                                    rtat_operation_t transa, rtat_operation_t transb, int m,
+                                    int n, int k, const float* alpha, const void* A, int lda,
+                                    const void* B, int ldb, rtat_activation_t act, const void* Z,
+                                    int ldz, const void* dD, int lddd,
+                                    const rtat_gemm_grads_t* grads);
+
+/* The step between two layers of a backward pass in one product:
+ *   D(m x n) = (alpha * op(A) * op(B)) * act'(Z) elementwise, dbias = row sums of D
+ * with A, B, Z and D of `type`; dbias (f32, m values, from the values before D is rounded) may be
+ * NULL.  D may be Z (same leading dimension).  dbias takes rtat_dbias_workspace_bytes(m, n) of
+ * the handle's scratch, as above. */
+rtat_status_t rtat_gemm_dact(rtat_handle_t handle, rtat_type_t type, rtat_operation_t transa,
+                             rtat_operation_t transb, int m, int n, int k, const float* alpha,
+                             const void* A, int lda, const void* B, int ldb,
+                             rtat_activation_t act, const void* Z, int ldz, void* D, int ldd,
+                             float* dbias);
+size_t rtat_dbias_workspace_bytes(int m, int n);
+
+/* Orthogonalises `batch` updates G_i (m x n, of g_type F32, F16 or BF16) into O_i (m x n, BF16):
+ *   X = G / (||G||_F + eps);  for each of `steps` triples (a, b, c) of `coeffs`:
+ *   M = X X^T,  X = a X + (b M + c M^2) X;   O = X
+ * (for m > n the same with M = X^T X).  coeffs is a host array of 3 * steps floats, read before
+ * the call returns; 1 <= steps <= RTAT_NEWTON_SCHULZ_MAX_STEPS.  Between products X and M are
+ * held in f16, scaled so that singular values up to 60 of X fit, and X in f32 as well until the
+ * last two steps, so O carries about nine bits: that is why it is BF16 whatever g_type is.
+ * G_i = G + i * stride_g, O_i = O + i * stride_o (elements; ignored when batch <= 1); O may be G
+ * when g_type is BF16 and the leading dimensions and strides agree.  An infinity or a NaN in G_i
+ * makes O_i NaN throughout and no other.
+ * Takes rtat_newton_schulz_workspace_bytes of the handle's scratch, as rtat_dtrsm does. */
+#define RTAT_NEWTON_SCHULZ_MAX_STEPS 32
+rtat_status_t rtat_newton_schulz(rtat_handle_t handle, rtat_type_t g_type, int m, int n,
+                                 int batch, const void* G, int ldg, int64_t stride_g, int steps,
+                                 const float* coeffs, float eps, void* O, int ldo,
+                                 int64_t stride_o);
+size_t rtat_newton_schulz_workspace_bytes(int m, int n, int batch);
+
 /* ---- operand generation -------------------------------------------------------------- */
 
 /* Kinds of synthetic operand. */

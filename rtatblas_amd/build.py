@@ -30,7 +30,8 @@ DEVICE_FLAGS = ["--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang"
 COMMON = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wextra", "-Wno-unused-parameter",
           "-I" + os.path.join(ROOT, "include")]
 
-NATIVE_SOURCES = ["api.hip", "geam.hip", "gemm.hip", "trsm.hip"]
+NATIVE_SOURCES = ["api.hip", "geam.hip", "gemm.hip", "gemm16.hip", "linear.hip", "orth.hip",
+                  "trsm.hip"]
 
 
 def _run(cmd):

@@ -2,6 +2,7 @@
 // checking, host-pointer scalars read by value, dispatch to the kernel launchers.
 #include <new>
 #include "common.h"
+#include "gemm16.h"
 
 #include <stdio.h>
 
@@ -89,6 +90,63 @@ void* acquire_workspace(rtat_native_handle* h, size_t bytes) {
 }
 
 }  // namespace rtat_native
+
+namespace {
+
+// The handle's device made current for the length of a call.
+struct OnDevice {
+  int before = -1;
+  explicit OnDevice(const rtat_native_handle* h) {
+    if (hipGetDevice(&before) != hipSuccess) {
+      (void)hipGetLastError();
+      before = -1;
+    }
+    if (before == h->device) before = -1;
+    else (void)hipSetDevice(h->device);
+  }
+  ~OnDevice() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+bool valid_half(int type) { return type == RTAT_TYPE_F16 || type == RTAT_TYPE_BF16; }
+bool valid_act(int act) { return act >= 0 && act < RTAT_ACT_COUNT; }
+bool short_ld(int ld, int rows) { return ld < (rows > 1 ? rows : 1); }
+
+// Shared checks of the 16-bit products: sizes, and the operands when they are read.
+rtat_status_t check_product(int type, int transa, int transb, int m, int n, int k,
+                            const float* alpha, const void* A, int lda, const void* B, int ldb) {
+  if (!valid_half(type) || !valid_op(transa) || !valid_op(transb)) return RTAT_STATUS_INVALID_ENUM;
+  if (m < 0 || n < 0 || k < 0 || alpha == nullptr) return RTAT_STATUS_INVALID_VALUE;
+  if (m == 0 || n == 0 || k == 0 || *alpha == 0.0f) return RTAT_STATUS_SUCCESS;
+  if (A == nullptr || B == nullptr || short_ld(lda, transa == RTAT_OP_T ? k : m) ||
+      short_ld(ldb, transb == RTAT_OP_T ? n : k))
+    return RTAT_STATUS_INVALID_VALUE;
+  return RTAT_STATUS_SUCCESS;
+}
+
+Gemm16 product(int type, bool ta, bool tb, int m, int n, int k, float alpha, const void* A,
+               long lda, const void* B, long ldb) {
+  Gemm16 g = {};
+  g.type = type;
+  g.ta = ta;
+  g.tb = tb;
+  g.m = m;
+  g.n = n;
+  g.k = alpha == 0.0f ? 0 : k;
+  g.batch = 1;
+  g.A = A;
+  g.lda = lda;
+  g.B = B;
+  g.ldb = ldb;
+  g.ep.rows = g.ep.c_rows = m;
+  g.ep.cols = g.ep.c_cols = n;
+  g.ep.alpha = alpha;
+  g.ep.bias_type = g.ep.aux_type = type;
+  return g;
+}
+
+}  // namespace
 
 #define RTAT_CHECK_HANDLE(h) \
   if ((h) == nullptr) return RTAT_STATUS_HANDLE_IS_NULLPTR
@@ -402,6 +460,166 @@ rtat_status_t rtat_hbm_probe(rtat_handle_t h, int kind, const void* src, void* d
                              size_t bytes) {
   RTAT_CHECK_HANDLE(h);
   return launch_probe(h, kind, src, dst, bytes);
+}
+
+rtat_status_t rtat_gemm_ep(rtat_handle_t h, rtat_type_t type, rtat_operation_t transa,
+                           rtat_operation_t transb, int m, int n, int k, const float* alpha,
+                           const void* A, int lda, const void* B, int ldb,
+                           const rtat_epilogue_t* ep, const float* beta, const void* C, int ldc,
+                           rtat_type_t d_type, void* D, int ldd) {
+  RTAT_CHECK_HANDLE(h);
+  rtat_status_t st = check_product(type, transa, transb, m, n, k, alpha, A, lda, B, ldb);
+  if (st != RTAT_STATUS_SUCCESS) return st;
+  if ((d_type != type && d_type != RTAT_TYPE_F32) || (ep != nullptr && !valid_act(ep->act)))
+    return RTAT_STATUS_INVALID_ENUM;
+  if (beta == nullptr) return RTAT_STATUS_INVALID_VALUE;
+  if (m == 0 || n == 0) return RTAT_STATUS_SUCCESS;
+  if (D == nullptr || short_ld(ldd, m)) return RTAT_STATUS_INVALID_VALUE;
+  if (*beta != 0.0f && (C == nullptr || short_ld(ldc, m))) return RTAT_STATUS_INVALID_VALUE;
+  if (ep != nullptr && ep->aux != nullptr && short_ld(ep->ldaux, m)) return RTAT_STATUS_INVALID_VALUE;
+  Gemm16 g = product(type, transa == RTAT_OP_T, transb == RTAT_OP_T, m, n, k, *alpha, A, lda, B, ldb);
+  if (ep != nullptr) {
+    g.ep.act = ep->act;
+    g.ep.bias = ep->bias;
+    g.ep.aux = ep->aux;
+    g.ep.ldaux = ep->ldaux;
+  }
+  g.ep.beta = *beta;
+  g.ep.C = *beta != 0.0f ? C : nullptr;
+  g.ep.ldc = ldc;
+  g.ep.c_type = g.ep.d_type = d_type;
+  g.ep.D = D;
+  g.ep.ldd = ldd;
+  OnDevice on(h);
+  return launch_gemm16(h, g);
+}
+
+rtat_status_t rtat_gemm_ep_backward(rtat_handle_t h, rtat_type_t type, rtat_operation_t transa,
+                                    rtat_operation_t transb, int m, int n, int k,
+                                    const float* alpha, const void* A, int lda, const void* B,
+                                    int ldb, rtat_activation_t act, const void* Z, int ldz,
+                                    const void* dD, int lddd, const rtat_gemm_grads_t* grads) {
+  RTAT_CHECK_HANDLE(h);
+  if (!valid_half(type) || !valid_op(transa) || !valid_op(transb) || !valid_act(act))
+    return RTAT_STATUS_INVALID_ENUM;
+  if (m < 0 || n < 0 || k < 0 || alpha == nullptr || grads == nullptr) return RTAT_STATUS_INVALID_VALUE;
+  const rtat_gemm_grads_t& q = *grads;
+  const bool ta = transa == RTAT_OP_T, tb = transb == RTAT_OP_T;
+  const bool want_a = q.dA != nullptr && m > 0 && k > 0, want_b = q.dB != nullptr && n > 0 && k > 0;
+  const bool slope = act != RTAT_ACT_NONE, some = m > 0 && n > 0;
+  if ((q.dA != nullptr && q.da_type != type && q.da_type != RTAT_TYPE_F32) ||
+      (q.dB != nullptr && q.db_type != type && q.db_type != RTAT_TYPE_F32))
+    return RTAT_STATUS_INVALID_ENUM;
+  if ((want_a && short_ld(q.ldda, ta ? k : m)) || (want_b && short_ld(q.lddb, tb ? n : k)))
+    return RTAT_STATUS_INVALID_VALUE;
+  if (some) {
+    if (dD == nullptr || short_ld(lddd, m)) return RTAT_STATUS_INVALID_VALUE;
+    if (slope && (Z == nullptr || short_ld(ldz, m))) return RTAT_STATUS_INVALID_VALUE;
+    if (slope && q.dZ != nullptr && short_ld(q.lddz, m)) return RTAT_STATUS_INVALID_VALUE;
+    if (*alpha != 0.0f) {
+      if (slope && q.dZ == nullptr && (want_a || want_b)) return RTAT_STATUS_INVALID_VALUE;
+      if (want_a && (B == nullptr || short_ld(ldb, tb ? n : k))) return RTAT_STATUS_INVALID_VALUE;
+      if (want_b && (A == nullptr || short_ld(lda, ta ? k : m))) return RTAT_STATUS_INVALID_VALUE;
+    }
+  }
+  OnDevice on(h);
+  rtat_status_t st = RTAT_STATUS_SUCCESS;
+  if (m > 0 && ((slope && q.dZ != nullptr && n > 0) || q.dbias != nullptr))
+    st = launch_act_backward(h, type, act, m, n, dD, lddd, Z, ldz, slope ? q.dZ : nullptr, q.lddz,
+                             q.dbias);
+  if (st != RTAT_STATUS_SUCCESS) return st;
+  const void* dZ = slope ? q.dZ : dD;
+  const long lddz = slope ? q.lddz : lddd;
+  if (want_a) {
+    // op(A) = A: dA (m x k) = dZ op(B)^T;  op(A) = A^T: dA (k x m) = op(B) dZ^T
+    Gemm16 g = ta ? product(type, tb, true, k, m, n, *alpha, B, ldb, dZ, lddz)
+                  : product(type, false, !tb, m, k, n, *alpha, dZ, lddz, B, ldb);
+    g.ep.beta = q.da_beta;
+    g.ep.C = q.da_beta != 0.0f ? q.dA : nullptr;
+    g.ep.D = q.dA;
+    g.ep.ldc = g.ep.ldd = q.ldda;
+    g.ep.c_type = g.ep.d_type = q.da_type;
+    st = launch_gemm16(h, g);
+    if (st != RTAT_STATUS_SUCCESS) return st;
+  }
+  if (want_b) {
+    // op(B) = B: dB (k x n) = op(A)^T dZ;  op(B) = B^T: dB (n x k) = dZ^T op(A)
+    Gemm16 g = tb ? product(type, true, ta, n, k, m, *alpha, dZ, lddz, A, lda)
+                  : product(type, !ta, false, k, n, m, *alpha, A, lda, dZ, lddz);
+    g.ep.beta = q.db_beta;
+    g.ep.C = q.db_beta != 0.0f ? q.dB : nullptr;
+    g.ep.D = q.dB;
+    g.ep.ldc = g.ep.ldd = q.lddb;
+    g.ep.c_type = g.ep.d_type = q.db_type;
+    st = launch_gemm16(h, g);
+  }
+  return st;
+}
+
+rtat_status_t rtat_gemm_dact(rtat_handle_t h, rtat_type_t type, rtat_operation_t transa,
+                             rtat_operation_t transb, int m, int n, int k, const float* alpha,
+                             const void* A, int lda, const void* B, int ldb,
+                             rtat_activation_t act, const void* Z, int ldz, void* D, int ldd,
+                             float* dbias) {
+  RTAT_CHECK_HANDLE(h);
+  rtat_status_t st = check_product(type, transa, transb, m, n, k, alpha, A, lda, B, ldb);
+  if (st != RTAT_STATUS_SUCCESS) return st;
+  if (!valid_act(act)) return RTAT_STATUS_INVALID_ENUM;
+  if (m == 0) return RTAT_STATUS_SUCCESS;
+  OnDevice on(h);
+  if (n == 0)  // sums over nothing
+    return dbias == nullptr ? RTAT_STATUS_SUCCESS : launch_sum_rows(h, nullptr, 0, m, dbias);
+  if (D == nullptr || short_ld(ldd, m)) return RTAT_STATUS_INVALID_VALUE;
+  if (act != RTAT_ACT_NONE && (Z == nullptr || short_ld(ldz, m))) return RTAT_STATUS_INVALID_VALUE;
+  Gemm16 g = product(type, transa == RTAT_OP_T, transb == RTAT_OP_T, m, n, k, *alpha, A, lda, B, ldb);
+  g.ep.slope = 1;
+  g.ep.act = act;
+  g.ep.aux = act != RTAT_ACT_NONE ? const_cast<void*>(Z) : nullptr;
+  g.ep.ldaux = ldz;
+  g.ep.D = D;
+  g.ep.ldd = ldd;
+  g.ep.d_type = type;
+  if (dbias == nullptr) return launch_gemm16(h, g);
+  g.ep.sums = static_cast<float*>(acquire_workspace(h, dbias_workspace_bytes(m, n)));
+  if (g.ep.sums == nullptr) return RTAT_STATUS_ALLOC_FAILED;
+  st = launch_gemm16(h, g);
+  if (st != RTAT_STATUS_SUCCESS) return st;
+  return launch_sum_rows(h, g.ep.sums, h->sum_rows, m, dbias);
+}
+
+size_t rtat_dbias_workspace_bytes(int m, int n) { return dbias_workspace_bytes(m, n); }
+
+rtat_status_t rtat_newton_schulz(rtat_handle_t h, rtat_type_t g_type, int m, int n, int batch,
+                                 const void* G, int ldg, int64_t stride_g, int steps,
+                                 const float* coeffs, float eps, void* O, int ldo,
+                                 int64_t stride_o) {
+  RTAT_CHECK_HANDLE(h);
+  if (!valid_half(g_type) && g_type != RTAT_TYPE_F32) return RTAT_STATUS_INVALID_ENUM;
+  if (m < 0 || n < 0 || batch < 0 || steps < 1 || steps > RTAT_NEWTON_SCHULZ_MAX_STEPS ||
+      coeffs == nullptr || !(eps >= 0.0f))
+    return RTAT_STATUS_INVALID_VALUE;
+  if (m == 0 || n == 0 || batch == 0) return RTAT_STATUS_SUCCESS;
+  if (G == nullptr || O == nullptr || short_ld(ldg, m) || short_ld(ldo, m))
+    return RTAT_STATUS_INVALID_VALUE;
+  if (batch > 65535) return RTAT_STATUS_INVALID_VALUE;  // a grid dimension
+  OnDevice on(h);
+  return launch_newton_schulz(h, g_type, m, n, batch, G, ldg, batch > 1 ? stride_g : 0, steps,
+                              coeffs, eps, O, ldo, batch > 1 ? stride_o : 0);
+}
+
+size_t rtat_newton_schulz_workspace_bytes(int m, int n, int batch) {
+  return newton_schulz_workspace_bytes(m, n, batch);
+}
+
+const char* rtat_activation_name(int act) {
+  switch (act) {
+    case RTAT_ACT_NONE: return "none";
+    case RTAT_ACT_RELU: return "relu";
+    case RTAT_ACT_GELU: return "gelu";
+    case RTAT_ACT_GELU_TANH: return "gelu_tanh";
+    case RTAT_ACT_SILU: return "silu";
+    default: return nullptr;
+  }
 }
 
 const char* rtat_version(void) { return "rtat-native 0.1 gfx950"; }

@@ -31,6 +31,8 @@ struct rtat_native_handle {
   void* static_ws = nullptr;
   // What the last GEMM-core launch on this handle did (rtat_last_launch).
   rtat_launch_info_t last = {};
+  // Rows of partial sums the last 16-bit gradient product left (Epilogue::sums).
+  int sum_rows = 0;
   int last_bm = 0, last_bn = 0;  // its tile shape; spelled into last.tile when asked for
 };
 

@@ -1,0 +1,295 @@
+// What the 16-bit products do to an element between the accumulator and memory: types,
+// activations and their derivatives, loads and stores of eight neighbouring elements.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "mfma.h"
+#include "rtat_native.h"
+
+namespace rtat_native {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef short s8_t __attribute__((ext_vector_type(8)));
+
+// The 16-bit operand types: eight of them as one MFMA operand, and the 16x16x32 MFMA.  Operand
+// lane l holds row (column) l % 16 and k = 8 * (l / 16) .. + 7; accumulator register r of lane l
+// holds D[4 * (l / 16) + r][l % 16].
+template <class T> struct Half;
+template <> struct Half<__bf16> {
+  typedef bf16x8_t vec_t;
+  static constexpr int id = RTAT_TYPE_BF16;
+  __device__ static inline f4_t mfma(s8_t a, s8_t b, f4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec_t, a),
+                                                   __builtin_bit_cast(vec_t, b), c, 0, 0, 0);
+  }
+};
+template <> struct Half<_Float16> {
+  typedef f16x8_t vec_t;
+  static constexpr int id = RTAT_TYPE_F16;
+  __device__ static inline f4_t mfma(s8_t a, s8_t b, f4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec_t, a),
+                                                  __builtin_bit_cast(vec_t, b), c, 0, 0, 0);
+  }
+};
+
+// Sixteen bytes at an address that is only element-aligned (one global load: the hardware
+// accepts any alignment).
+struct __attribute__((packed, aligned(2))) Loose16 {
+  u4_t v;
+};
+
+__device__ inline float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896f); }
+__device__ inline float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// Phi(z) and the density phi(z) of the normal distribution.  erfc by Abramowitz and Stegun 7.1.26
+// (a quintic in t = 1 / (1 + p x) times exp(-x^2), off by at most 1.5e-7), x = |z| / sqrt 2, so
+// that one exponential serves both.
+__device__ inline void normal_cdf(float z, float& Phi, float& phi) {
+  const float x = __builtin_fabsf(z) * 0.707106781186548f;
+  const float e = exp_fast(-x * x);
+  const float t = rcp_fast(__builtin_fmaf(0.3275911f, x, 1.0f));
+  float q = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  q = __builtin_fmaf(q, t, 1.421413741f);
+  q = __builtin_fmaf(q, t, -0.284496736f);
+  q = __builtin_fmaf(q, t, 0.254829592f);
+  const float half_erfc = 0.5f * q * t * e;
+  Phi = z < 0.0f ? half_erfc : 1.0f - half_erfc;
+  phi = 0.398942280401433f * e;
+}
+
+// u of GELU_TANH with the factor two that turns (1 + tanh u) / 2 into a logistic of 2u.
+constexpr float GELU_C2 = 1.59576912160573f;  // 2 sqrt(2 / pi)
+constexpr float GELU_K = 0.044715f;
+
+__device__ inline float act_value(int act, float z) {
+  switch (act) {
+    case RTAT_ACT_RELU: return z < 0.0f ? 0.0f : z;
+    case RTAT_ACT_GELU: {
+      float Phi, phi;
+      normal_cdf(z, Phi, phi);
+      return z * Phi;
+    }
+    case RTAT_ACT_GELU_TANH: return z * rcp_fast(1.0f + exp_fast(-GELU_C2 * z * __builtin_fmaf(GELU_K * z, z, 1.0f)));
+    case RTAT_ACT_SILU: return z * rcp_fast(1.0f + exp_fast(-z));
+    default: return z;
+  }
+}
+
+// Past +-100 every slope is 0 or 1 to the last bit; the bound keeps infinities and squares that
+// overflow out of products with 0.  A NaN stays one.
+__device__ inline float act_slope(int act, float z) {
+  if (act != RTAT_ACT_RELU) z = z > 100.0f ? 100.0f : (z < -100.0f ? -100.0f : z);
+  switch (act) {
+    case RTAT_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+    case RTAT_ACT_GELU: {
+      float Phi, phi;
+      normal_cdf(z, Phi, phi);
+      return __builtin_fmaf(z, phi, Phi);
+    }
+    case RTAT_ACT_GELU_TANH: {
+      const float z2 = z * z;
+      const float p = rcp_fast(1.0f + exp_fast(-GELU_C2 * z * __builtin_fmaf(GELU_K, z2, 1.0f)));
+      // d(2u)/dz = 2 sqrt(2/pi) (1 + 3 * 0.044715 z^2)
+      return p + z * GELU_C2 * __builtin_fmaf(3.0f * GELU_K, z2, 1.0f) * (p * (1.0f - p));
+    }
+    case RTAT_ACT_SILU: {
+      const float p = rcp_fast(1.0f + exp_fast(-z));
+      return p * __builtin_fmaf(z, 1.0f - p, 1.0f);
+    }
+    default: return 1.0f;
+  }
+}
+
+__host__ __device__ inline int type_bytes(int type) { return type == RTAT_TYPE_F32 ? 4 : 2; }
+
+__device__ inline float half_to_float(int type, uint16_t bits) {
+  return type == RTAT_TYPE_BF16 ? (float)__builtin_bit_cast(__bf16, bits)
+                                : (float)__builtin_bit_cast(_Float16, bits);
+}
+// Rounds to nearest even.
+__device__ inline uint16_t float_to_half(int type, float x) {
+  return type == RTAT_TYPE_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)x)
+                                : __builtin_bit_cast(uint16_t, (_Float16)x);
+}
+
+__device__ inline float load_one(int type, const void* p, long i) {
+  return type == RTAT_TYPE_F32 ? static_cast<const float*>(p)[i]
+                               : half_to_float(type, static_cast<const uint16_t*>(p)[i]);
+}
+__device__ inline void store_one(int type, void* p, long i, float x) {
+  if (type == RTAT_TYPE_F32) static_cast<float*>(p)[i] = x;
+  else static_cast<uint16_t*>(p)[i] = float_to_half(type, x);
+}
+
+// Eight neighbours on a 16-byte boundary.
+__device__ inline void unpack8(int type, u4_t raw, float (&v)[8]) {
+  if (type == RTAT_TYPE_BF16) {
+    const bf16x8_t h = __builtin_bit_cast(bf16x8_t, raw);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)h[e];
+  } else {
+    const f16x8_t h = __builtin_bit_cast(f16x8_t, raw);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)h[e];
+  }
+}
+__device__ inline u4_t pack8(int type, const float (&v)[8]) {
+  if (type == RTAT_TYPE_BF16) {
+    bf16x8_t h;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = (__bf16)v[e];
+    return __builtin_bit_cast(u4_t, h);
+  }
+  f16x8_t h;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) h[e] = (_Float16)v[e];
+  return __builtin_bit_cast(u4_t, h);
+}
+__device__ inline void load8(int type, const void* p, long i, float (&v)[8]) {
+  if (type == RTAT_TYPE_F32) {
+    const f4_t* q = reinterpret_cast<const f4_t*>(static_cast<const float*>(p) + i);
+    const f4_t a = q[0], b = q[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = a[e];
+      v[4 + e] = b[e];
+    }
+  } else {
+    unpack8(type, *reinterpret_cast<const u4_t*>(static_cast<const uint16_t*>(p) + i), v);
+  }
+}
+__device__ inline void store8(int type, void* p, long i, const float (&v)[8]) {
+  if (type == RTAT_TYPE_F32) {
+    f4_t* q = reinterpret_cast<f4_t*>(static_cast<float*>(p) + i);
+    f4_t a, b;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      a[e] = v[e];
+      b[e] = v[4 + e];
+    }
+    q[0] = a;
+    q[1] = b;
+  } else {
+    *reinterpret_cast<u4_t*>(static_cast<uint16_t*>(p) + i) = pack8(type, v);
+  }
+}
+
+// What becomes of the product.  Elements (row, col) with row < rows and col < cols are stored.
+//   forward (slope == 0): z = alpha * acc + bias[row]; aux = z; D = act(z) + beta * C
+//   gradient (slope == 1): D = alpha * acc * act'(aux); sums += D along the columns
+// C counts as zero outside c_rows x c_cols.  `copy` receives what D does, in f16.  `scale`, if
+// given, points to a pair (r, e) per matrix of a batch on the device: alpha is multiplied by
+// r^r_power and, when scale_c, C is read as r * 2^e * C.
+struct Epilogue {
+  int rows, cols;
+  int act, slope;
+  float alpha, beta;
+  const void* bias;
+  int bias_type;
+  void* aux;
+  long ldaux, aux_stride;
+  int aux_type;
+  const void* C;
+  long ldc, c_stride;
+  int c_type, c_rows, c_cols;
+  void* D;
+  long ldd, d_stride;
+  int d_type;
+  void* copy;
+  long ldcopy, copy_stride;
+  float* sums;  // gradient: one row of `rows` partial sums per wave column of the launch
+  const float* scale;
+  int r_power, scale_c;
+  int vec;  // 1: bias, aux, C and D may be accessed sixteen bytes at a time at rows 8 i
+};
+
+// Sixteen-byte access at rows that are multiples of eight: base and column stride in bytes
+// (and the batch's) are multiples of 16.
+inline bool vec_ok(const void* p, long ld, long stride, int type) {
+  const long es = type_bytes(type);
+  return p == nullptr || ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * es) | (uintptr_t)(stride * es)) & 15) == 0;
+}
+inline void settle_vec(Epilogue& e) {
+  e.vec = vec_ok(e.bias, 0, 0, e.bias_type) && vec_ok(e.aux, e.ldaux, e.aux_stride, e.aux_type) &&
+          vec_ok(e.C, e.ldc, e.c_stride, e.c_type) &&
+          vec_ok(e.copy, e.ldcopy, e.copy_stride, RTAT_TYPE_F16) && vec_ok(e.D, e.ldd, e.d_stride, e.d_type);
+}
+
+// Rows row .. row + 7 of column col, batch matrix z: v holds the accumulators and, for a
+// gradient, leaves with the values that belong to the row sums (0 outside).
+__device__ inline void epilogue8(const Epilogue& e, float alpha, float beta, int c_exp, int row,
+                                 int col, long z, float (&v)[8]) {
+  if (col >= e.cols || row >= e.rows) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    return;
+  }
+  const long d_at = z * e.d_stride + row + (long)col * e.ldd;
+  const long aux_at = z * e.aux_stride + row + (long)col * e.ldaux;
+  const long c_at = z * e.c_stride + row + (long)col * e.ldc;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] *= alpha;
+  if (e.vec && row + 8 <= e.rows && (e.C == nullptr || row + 8 <= e.c_rows)) {
+    float w[8];
+    if (e.slope) {
+      if (e.act != RTAT_ACT_NONE) {
+        load8(e.aux_type, e.aux, aux_at, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= act_slope(e.act, w[i]);
+      }
+    } else {
+      float c[8];
+      const bool with_c = e.C != nullptr && col < e.c_cols;
+      if (with_c) load8(e.c_type, e.C, c_at, c);
+      if (e.bias != nullptr) {
+        load8(e.bias_type, e.bias, row, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += w[i];
+      }
+      if (e.aux != nullptr) store8(e.aux_type, e.aux, aux_at, v);
+      if (e.act != RTAT_ACT_NONE) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = act_value(e.act, v[i]);
+      }
+      if (with_c) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          v[i] = __builtin_fmaf(beta, c_exp ? __builtin_ldexpf(c[i], c_exp) : c[i], v[i]);
+      }
+    }
+    store8(e.d_type, e.D, d_at, v);
+    if (e.copy != nullptr)
+      store8(RTAT_TYPE_F16, e.copy, z * e.copy_stride + row + (long)col * e.ldcopy, v);
+    return;
+  }
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    // v is indexed by a constant in every copy of this body: no scratch memory.
+    float x = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) x = q == i ? v[q] : x;
+    if (row + i < e.rows) {
+      if (e.slope) {
+        if (e.act != RTAT_ACT_NONE) x *= act_slope(e.act, load_one(e.aux_type, e.aux, aux_at + i));
+      } else {
+        if (e.bias != nullptr) x += load_one(e.bias_type, e.bias, row + i);
+        if (e.aux != nullptr) store_one(e.aux_type, e.aux, aux_at + i, x);
+        x = act_value(e.act, x);
+        if (e.C != nullptr && row + i < e.c_rows && col < e.c_cols)
+          x = __builtin_fmaf(beta, __builtin_ldexpf(load_one(e.c_type, e.C, c_at + i), c_exp), x);
+      }
+      store_one(e.d_type, e.D, d_at + i, x);
+      if (e.copy != nullptr)
+        store_one(RTAT_TYPE_F16, e.copy, z * e.copy_stride + row + (long)col * e.ldcopy + i, x);
+    } else {
+      x = 0.0f;
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = q == i ? x : v[q];
+  }
+}
+
+}  // namespace rtat_native

@@ -1,0 +1,355 @@
+// Products of 16-bit matrices on the matrix cores (v_mfma_f32_16x16x32_{bf16,f16}) with an
+// elementwise epilogue, for the linear layer's forward and backward passes and for the
+// Newton-Schulz iteration.  Column-major, D(m x n) = epilogue(op(A) op(B)); f32 accumulation.
+//
+//   * One workgroup computes a BM x BN tile; K advances BK = 64 elements (128 bytes) at a time
+//     through two LDS stages.
+//   * Panels keep the orientation they have in memory.  An operand that is contiguous along k
+//     ("k-major") lies as rows of 64 k, one 16-byte read per lane and MFMA operand; one that is
+//     contiguous along m / n ("mn-major") lies as 64 rows of BM (BN) elements and is read with
+//     the transposing LDS load (ds_read_b64_tr_b16: lane i of a group of 16 gets column i of the
+//     4 x 16 block that the group addresses), two reads per operand.
+//   * Sixteen-byte chunks of a panel row are permuted by an XOR of the row number, which spreads
+//     each read over the LDS banks.  Measured clocks per wave instruction, 16 waves of a CU
+//     reading: 16 bytes per lane 3.8 with it, 10.3 without; transposing 2.9 with it, 11.0
+//     without (row strides of 128 and 512 bytes).
+//   * The accumulators pass through LDS one block column at a time, which turns them into eight
+//     neighbouring rows per lane: bias, residual, saved activations and results move in 16-byte
+//     accesses, and the epilogue is one rolled loop whatever it has to do.
+#include <type_traits>
+
+#include "gemm16.h"
+#include "gemm_plan.h"
+
+namespace rtat_native {
+
+namespace {
+
+struct Gemm16Args {
+  int m, n, k, tri;
+  int tiles_m, tiles_n, tiles;  // tiles per matrix of the batch
+  const uint16_t* A;
+  long lda, a_stride;
+  const uint16_t* B;
+  long ldb, b_stride;
+  Epilogue ep;
+};
+
+constexpr int BK16 = 64;
+
+template <int BM_, int BN_, int WGM_, int WGN_, int OCC_>
+struct Shape16 {
+  static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, OCC = OCC_;
+  static constexpr int NW = WGM * WGN, NT = 64 * NW;
+  static constexpr int WTM = BM / WGM, WTN = BN / WGN;  // wave tile
+  static constexpr int TM = WTM / 16, TN = WTN / 16;    // MFMA blocks per wave tile
+  static constexpr int STAGE = (BM + BN) * BK16 * 2;    // bytes
+  static constexpr int PARK = WTM + 4;                  // floats per parked column
+  static constexpr int LDS = 2 * STAGE > NW * 16 * PARK * 4 ? 2 * STAGE : NW * 16 * PARK * 4;
+};
+
+// A panel of ROWS x 64 elements in LDS, in bytes.
+template <bool KMAJOR, int ROWS>
+struct Panel16 {
+  static constexpr int BYTES = ROWS * BK16 * 2;
+  static constexpr int ROWBYTES = KMAJOR ? 128 : ROWS * 2;
+  static constexpr int CHUNKS = ROWBYTES / 16;
+  // What the chunk index of LDS row r is XORed with.  k-major: eight rows, eight chunks.
+  // mn-major: a transposing read takes 32 bytes of each of the rows k = 8 q + 0 .. 3 for two
+  // neighbouring q at a time; rows of 256 bytes or more all start at the same bank, 128-byte rows
+  // alternate between two.
+  __device__ static inline int key(int r) {
+    if (KMAJOR) return r & 7;
+    if (ROWS >= 128) return 2 * ((r & 3) | ((r >> 1) & 4));
+    return 2 * (((r >> 1) & 1) | ((r >> 2) & 2));
+  }
+  // Chunk c (of the panel, in LDS order) holds elements of LDS row c / CHUNKS, from element
+  // 8 * source_chunk(c).
+  __device__ static inline int source_chunk(int c) {
+    const int r = c / CHUNKS;
+    return (c % CHUNKS) ^ key(r);
+  }
+};
+
+// Fragments of MFMA K-step `step` (0 or 1) for TB blocks of 16 rows starting at row w0.
+template <bool KMAJOR, int ROWS, int TB>
+__device__ inline void read_frags(const unsigned char* panel, int w0, int step, int lane,
+                                  s8_t (&f)[TB]) {
+  typedef Panel16<KMAJOR, ROWS> P;
+  const int l16 = lane & 15, q = lane >> 4;
+  if constexpr (KMAJOR) {
+    const int chunk = (4 * step + q) ^ P::key(l16);
+    const unsigned char* at = panel + (w0 + l16) * P::ROWBYTES + chunk * 16;
+#pragma unroll
+    for (int b = 0; b < TB; ++b) f[b] = *reinterpret_cast<const s8_t*>(at + b * 16 * P::ROWBYTES);
+  } else {
+    typedef __attribute__((address_space(3))) s4_t* lds4_t;
+    // Lane j of a group addresses 4 elements at row k = 8 q + j / 4 (and + 4), column 4 (j % 4).
+    const int k = 32 * step + 8 * q + (l16 >> 2), key = P::key(k & 15);
+    const unsigned char* row = panel + k * P::ROWBYTES + (l16 & 1) * 8;
+#pragma unroll
+    for (int b = 0; b < TB; ++b) {
+      const int chunk = (w0 / 8 + 2 * b + ((l16 >> 1) & 1)) ^ key;
+      const unsigned char* at = row + chunk * 16;
+      const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(at));
+      const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(at + 4 * P::ROWBYTES));
+      f[b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+}
+
+// Global -> register -> LDS mover of one panel: any alignment, leading dimension and edge.
+// Rows past row_lim repeat the last one (they reach accumulators that are not stored), k past
+// k_lim reads as zero.
+template <bool KMAJOR, int ROWS, int NT>
+struct Mover16 {
+  typedef Panel16<KMAJOR, ROWS> P;
+  static constexpr int NV = P::BYTES / (16 * NT);
+  u4_t r[NV];
+
+  __device__ inline void load(const uint16_t* base, long ld, int row0, int row_lim, int k0,
+                              int k_lim, int t) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = i * NT + t, lr = c / P::CHUNKS, e0 = P::source_chunk(c) * 8;
+      int row = KMAJOR ? row0 + lr : row0 + e0;
+      const int k = KMAJOR ? k0 + e0 : k0 + lr;
+      bool whole;
+      if constexpr (KMAJOR) {
+        row = row < row_lim ? row : row_lim - 1;
+        whole = k + 8 <= k_lim;
+      } else {
+        whole = k < k_lim && row + 8 <= row_lim;
+      }
+      const uint16_t* at = KMAJOR ? base + (long)row * ld + k : base + (long)k * ld + row;
+      if (whole) {
+        r[i] = reinterpret_cast<const Loose16*>(at)->v;
+      } else {
+        s8_t v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool in = KMAJOR ? k + e < k_lim : (k < k_lim && row + e < row_lim);
+          v[e] = in ? (short)at[e] : (short)0;
+        }
+        r[i] = __builtin_bit_cast(u4_t, v);
+      }
+    }
+  }
+  __device__ inline void store(unsigned char* panel, int t) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) *reinterpret_cast<u4_t*>(panel + (i * NT + t) * 16) = r[i];
+  }
+};
+
+template <class T, class S, bool KA, bool KB>
+__global__ __launch_bounds__(S::NT, S::OCC) void gemm16_kernel(Gemm16Args p) {
+  constexpr int TM = S::TM, TN = S::TN;
+  extern __shared__ __align__(16) unsigned char lds[];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int wm0 = (wave % S::WGM) * S::WTM, wn0 = (wave / S::WGM) * S::WTN;
+
+  const int logical = logical_of_workgroup(blockIdx.x, gridDim.x);
+  const long z = logical / p.tiles;
+  int tile_m, tile_n;
+  tile_of_logical(logical % p.tiles, p.tiles_m, p.tiles_n, p.tri, S::BM, S::BN, tile_m, tile_n);
+  const int m0 = tile_m * S::BM, n0 = tile_n * S::BN;
+  const uint16_t* A = p.A + z * p.a_stride;
+  const uint16_t* B = p.B + z * p.b_stride;
+
+  f4_t acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{0, 0, 0, 0};
+
+  const int panels = (p.k + BK16 - 1) / BK16;
+  typedef Panel16<KA, S::BM> PA;
+  Mover16<KA, S::BM, S::NT> ma;
+  Mover16<KB, S::BN, S::NT> mb;
+  auto load = [&](int kt) {
+    ma.load(A, p.lda, m0, p.m, kt * BK16, p.k, t);
+    mb.load(B, p.ldb, n0, p.n, kt * BK16, p.k, t);
+  };
+  auto store = [&](int kt) {
+    unsigned char* stage = lds + (kt & 1) * S::STAGE;
+    ma.store(stage, t);
+    mb.store(stage + PA::BYTES, t);
+  };
+  if (panels > 0) {
+    load(0);
+    store(0);
+    if (panels > 1) load(1);
+  }
+  __syncthreads();
+  for (int kt = 0; kt < panels; ++kt) {
+    const unsigned char* stage = lds + (kt & 1) * S::STAGE;
+    if (kt + 1 < panels) store(kt + 1);
+    if (kt + 2 < panels) load(kt + 2);
+#pragma unroll
+    for (int step = 0; step < 2; ++step) {
+      s8_t fa[TM], fb[TN];
+      read_frags<KA, S::BM>(stage, wm0, step, lane, fa);
+      read_frags<KB, S::BN>(stage + PA::BYTES, wn0, step, lane, fb);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = Half<T>::mfma(fa[i], fb[j], acc[i][j]);
+    }
+    __syncthreads();
+  }
+
+  // Epilogue, a block column (16 columns of C) at a time: the wave parks it in its own part of
+  // LDS, column by column, and takes it back as eight neighbouring rows per lane.
+  const Epilogue& e = p.ep;
+  float alpha = e.alpha, beta = e.beta;
+  int c_exp = 0;
+  if (e.scale != nullptr) {
+    const float r = e.scale[2 * z];
+    for (int i = 0; i < e.r_power; ++i) alpha *= r;
+    if (e.scale_c) {
+      beta *= r;
+      c_exp = (int)e.scale[2 * z + 1];
+    }
+  }
+  float* park = reinterpret_cast<float*>(lds) + wave * 16 * S::PARK;
+  constexpr int LPC = S::WTM / 8;   // lanes per column
+  constexpr int CPP = 64 / LPC;     // columns per pass
+  const int er = (lane % LPC) * 8;  // row of this lane inside the wave tile
+  float sums[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sums[i] = 0.0f;
+  const bool mirror = p.tri != 0 && tile_m != tile_n;
+#pragma unroll 1
+  for (int j = 0; j < TN; ++j) {
+#pragma unroll
+    for (int jj = 0; jj < TN; ++jj)
+      if (jj == j) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+          *reinterpret_cast<f4_t*>(park + (lane & 15) * S::PARK + 16 * i + 4 * (lane >> 4)) =
+              acc[i][jj];
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int c0 = 0; c0 < 16; c0 += CPP) {
+      const int c = c0 + lane / LPC;
+      const f4_t* at = reinterpret_cast<const f4_t*>(park + c * S::PARK + er);
+      const f4_t lo = at[0], hi = at[1];
+      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      epilogue8(e, alpha, beta, c_exp, m0 + wm0 + er, n0 + wn0 + 16 * j + c, z, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sums[i] += v[i];
+    }
+    if (mirror) {
+      // The same 16 columns as rows of the mirrored tile: lane pairs take the two halves.
+#pragma unroll 1
+      for (int r0 = 0; r0 < S::WTM; r0 += 32) {
+        const int r = r0 + (lane >> 1), c = 8 * (lane & 1);
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = park[(c + i) * S::PARK + r];
+        epilogue8(e, alpha, beta, c_exp, n0 + wn0 + 16 * j + c, m0 + wm0 + r, z, v);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  if (e.sums != nullptr) {
+    // Lanes with the same rows add up in a fixed order; one partial row per wave column.
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int d = LPC; d < 64; d *= 2) sums[i] += __shfl_xor(sums[i], d);
+    if (lane < LPC) {
+      float* out = e.sums + (long)(tile_n * S::WGN + wave / S::WGM) * e.rows;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (m0 + wm0 + er + i < e.rows) out[m0 + wm0 + er + i] = sums[i];
+    }
+  }
+}
+
+typedef Shape16<128, 128, 2, 2, 2> S128x128;
+typedef Shape16<64, 64, 2, 2, 4> S64x64;
+
+template <class T, class S, bool KA, bool KB>
+rtat_status_t launch_shape(rtat_native_handle* h, const Gemm16& g, Gemm16Args p) {
+  static PerDeviceOnce configured;
+  auto kern = gemm16_kernel<T, S, KA, KB>;
+  if (!configured(h->device, [&] {
+        if (S::LDS <= 65536) return true;
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS) == hipSuccess)
+          return true;
+        (void)hipGetLastError();
+        return false;
+      }))
+    return RTAT_STATUS_NOT_SUPPORTED;
+  p.tiles_m = (p.m + S::BM - 1) / S::BM;
+  p.tiles_n = (p.n + S::BN - 1) / S::BN;
+  const long tiles = p.tri != 0 ? (long)p.tiles_m * (p.tiles_m + 1) / 2 : (long)p.tiles_m * p.tiles_n;
+  if (tiles * g.batch > 0x7fffffffL) return RTAT_STATUS_INVALID_VALUE;
+  p.tiles = (int)tiles;
+  h->sum_rows = p.tiles_n * S::WGN;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(tiles * g.batch)), dim3(S::NT), S::LDS, h->stream, p);
+  return launch_status();
+}
+
+template <class T, class S>
+rtat_status_t launch_ops16(rtat_native_handle* h, const Gemm16& g, const Gemm16Args& p) {
+  const bool ka = g.ta, kb = !g.tb;  // contiguous along k
+  if (ka && kb) return launch_shape<T, S, true, true>(h, g, p);
+  if (ka) return launch_shape<T, S, true, false>(h, g, p);
+  if (kb) return launch_shape<T, S, false, true>(h, g, p);
+  return launch_shape<T, S, false, false>(h, g, p);
+}
+
+template <class T>
+rtat_status_t launch_type(rtat_native_handle* h, const Gemm16& g, const Gemm16Args& p) {
+  const long cus = h->compute_units > 0 ? h->compute_units : 256;
+  const long big = (long)((p.m + 127) / 128) * ((p.n + 127) / 128) * g.batch / (p.tri ? 2 : 1);
+  if (big >= cus) return launch_ops16<T, S128x128>(h, g, p);
+  return launch_ops16<T, S64x64>(h, g, p);
+}
+
+__global__ __launch_bounds__(256) void sum_rows_kernel(const float* parts, int count, int m,
+                                                       float* out) {
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  if (row >= m) return;
+  float s = 0.0f;
+#pragma unroll 8
+  for (int i = 0; i < count; ++i) s += parts[(long)i * m + row];
+  out[row] = s;
+}
+
+}  // namespace
+
+int dact_sum_rows(int n) { return 2 * ((n + 63) / 64); }
+
+rtat_status_t launch_sum_rows(rtat_native_handle* h, const float* parts, int count, int m,
+                              float* out) {
+  hipLaunchKernelGGL(sum_rows_kernel, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, h->stream,
+                     parts, count, m, out);
+  return launch_status();
+}
+
+rtat_status_t launch_gemm16(rtat_native_handle* h, const Gemm16& g) {
+  if (g.m <= 0 || g.n <= 0 || g.batch <= 0) return RTAT_STATUS_SUCCESS;
+  Gemm16Args p = {};
+  p.m = g.m;
+  p.n = g.n;
+  p.k = g.k;
+  p.tri = g.tri;
+  p.A = static_cast<const uint16_t*>(g.A);
+  p.lda = g.lda;
+  p.a_stride = g.a_stride;
+  p.B = static_cast<const uint16_t*>(g.B);
+  p.ldb = g.ldb;
+  p.b_stride = g.b_stride;
+  p.ep = g.ep;
+  settle_vec(p.ep);
+  return g.type == RTAT_TYPE_BF16 ? launch_type<__bf16>(h, g, p) : launch_type<_Float16>(h, g, p);
+}
+
+}  // namespace rtat_native

@@ -29,6 +29,11 @@ def kernel_options(tile=GEMM_AUTO, tail=TAIL_AUTO, panel=PANEL_AUTO):
 PROBE_READ, PROBE_WRITE, PROBE_COPY = 0, 1, 2
 FILL_IID, FILL_SYMMETRIC, FILL_TRI_LOWER, FILL_UNIT_INTERVAL, FILL_TRI_FULL = 0, 1, 2, 3, 4
 
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 2, 14
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = 0, 1, 2, 3, 4
+ACT_COUNT = 5
+NEWTON_SCHULZ_MAX_STEPS = 32
+
 STATUS_NAMES = {0: "SUCCESS", 1: "NOT_INITIALIZED", 2: "ALLOC_FAILED", 3: "INVALID_VALUE",
                 5: "EXECUTION_FAILED", 7: "NOT_SUPPORTED", 9: "HANDLE_IS_NULLPTR",
                 10: "INVALID_ENUM"}
@@ -65,6 +70,17 @@ SIGNATURES = {
     "rtat_sgemm_ex": (_i, [_vp, _i, _i, _i, _i, _i, _pf, _vp, _i, _vp, _i, _pf, _vp, _i, _i]),
     "rtat_ssyrk_ex": (_i, [_vp, _i, _i, _i, _i, _pf, _vp, _i, _pf, _vp, _i, _i]),
     "rtat_strsm_ex": (_i, [_vp, _i, _i, _i, _i, _i, _i, _pf, _vp, _i, _vp, _i, _i]),
+    "rtat_activation_name": (C.c_char_p, [_i]),
+    "rtat_gemm_ep": (_i, [_vp, _i, _i, _i, _i, _i, _i, _pf, _vp, _i, _vp, _i, _vp, _pf, _vp, _i,
+                          _i, _vp, _i]),
+    "rtat_gemm_ep_backward": (_i, [_vp, _i, _i, _i, _i, _i, _i, _pf, _vp, _i, _vp, _i, _i, _vp,
+                                   _i, _vp, _i, _vp]),
+    "rtat_gemm_dact": (_i, [_vp, _i, _i, _i, _i, _i, _i, _pf, _vp, _i, _vp, _i, _i, _vp, _i, _vp,
+                            _i, _vp]),
+    "rtat_dbias_workspace_bytes": (C.c_size_t, [_i, _i]),
+    "rtat_newton_schulz": (_i, [_vp, _i, _i, _i, _i, _vp, _i, C.c_int64, _i, _pf, C.c_float, _vp,
+                                _i, C.c_int64]),
+    "rtat_newton_schulz_workspace_bytes": (C.c_size_t, [_i, _i, _i]),
     "rtat_dfill": (_i, [_vp, _vp, _i, _i, _i, C.c_uint64, _i]),
     "rtat_sfill": (_i, [_vp, _vp, _i, _i, _i, C.c_uint64, _i]),
     "rtat_device_peaks": (_i, [_vp, _pd, _pd, C.POINTER(_i)]),
@@ -84,6 +100,18 @@ class Move(C.Structure):
     """rtat_move_t: one job of rtat_dmove_pair / rtat_smove_pair."""
     _fields_ = [("trans", _i), ("m", _i), ("n", _i), ("A", _vp), ("lda", _i), ("C", _vp),
                 ("ldc", _i)]
+
+
+class EpilogueArgs(C.Structure):
+    """rtat_epilogue_t."""
+    _fields_ = [("act", _i), ("bias", _vp), ("aux", _vp), ("ldaux", _i)]
+
+
+class GemmGrads(C.Structure):
+    """rtat_gemm_grads_t."""
+    _fields_ = [("dZ", _vp), ("lddz", _i), ("da_type", _i), ("da_beta", C.c_float), ("dA", _vp),
+                ("ldda", _i), ("db_type", _i), ("db_beta", C.c_float), ("dB", _vp), ("lddb", _i),
+                ("dbias", _vp)]
 
 
 _lib = None
@@ -124,6 +152,13 @@ def _ptr(x):
     if isinstance(x, int):
         return x
     return x.data_ptr()
+
+
+def _f(x):
+    return C.byref(C.c_float(x))
+
+
+_ref = C.byref
 
 
 class Handle:
@@ -243,6 +278,52 @@ class Handle:
             _check("rtat_sgeam", st)
         return st
 
+    def gemm_ep(self, type, ta, tb, m, n, k, alpha, A, lda, B, ldb, D, ldd, d_type=None,
+                act=ACT_NONE, bias=None, aux=None, ldaux=0, beta=0.0, C=None, ldc=0, check=True):
+        """D = act(alpha*op(A)*op(B) + bias) + beta*C; d_type defaults to the operands' type."""
+        ep = EpilogueArgs(act, _ptr(bias), _ptr(aux), ldaux)
+        st = self.lib.rtat_gemm_ep(self.h, type, ta, tb, m, n, k, _f(alpha), _ptr(A), lda,
+                                   _ptr(B), ldb, _ref(ep), _f(beta), _ptr(C), ldc,
+                                   type if d_type is None else d_type, _ptr(D), ldd)
+        if check:
+            _check("rtat_gemm_ep", st)
+        return st
+
+    def gemm_ep_backward(self, type, ta, tb, m, n, k, alpha, A, lda, B, ldb, dD, lddd,
+                         act=ACT_NONE, aux=None, ldaux=0, dZ=None, lddz=0, dA=None, ldda=0,
+                         da_type=None, da_beta=0.0, dB=None, lddb=0, db_type=None, db_beta=0.0,
+                         dbias=None, check=True):
+        """Gradients of gemm_ep; aux is what the forward call left there."""
+        g = GemmGrads(_ptr(dZ), lddz, type if da_type is None else da_type, da_beta, _ptr(dA),
+                      ldda, type if db_type is None else db_type, db_beta, _ptr(dB), lddb,
+                      _ptr(dbias))
+        st = self.lib.rtat_gemm_ep_backward(self.h, type, ta, tb, m, n, k, _f(alpha), _ptr(A),
+                                            lda, _ptr(B), ldb, act, _ptr(aux), ldaux, _ptr(dD),
+                                            lddd, _ref(g))
+        if check:
+            _check("rtat_gemm_ep_backward", st)
+        return st
+
+    def gemm_dact(self, type, ta, tb, m, n, k, alpha, A, lda, B, ldb, act, Z, ldz, D, ldd,
+                  dbias=None, check=True):
+        """D = (alpha*op(A)*op(B)) * act'(Z), dbias = row sums of D (f32)."""
+        st = self.lib.rtat_gemm_dact(self.h, type, ta, tb, m, n, k, _f(alpha), _ptr(A), lda,
+                                     _ptr(B), ldb, act, _ptr(Z), ldz, _ptr(D), ldd, _ptr(dbias))
+        if check:
+            _check("rtat_gemm_dact", st)
+        return st
+
+    def newton_schulz(self, g_type, m, n, G, ldg, O, ldo, coeffs, eps=1e-7, batch=1, strideg=0,
+                      strideo=0, check=True):
+        """Orthogonalises G into O (bf16) by len(coeffs) steps of (a, b, c)."""
+        flat = [x for step in coeffs for x in step]
+        arr = (C.c_float * max(len(flat), 1))(*flat)
+        st = self.lib.rtat_newton_schulz(self.h, g_type, m, n, batch, _ptr(G), ldg, strideg,
+                                         len(coeffs), arr, eps, _ptr(O), ldo, strideo)
+        if check:
+            _check("rtat_newton_schulz", st)
+        return st
+
     def dfill(self, A, m, n, ld, seed, kind=FILL_IID, check=True):
         st = self.lib.rtat_dfill(self.h, _ptr(A), m, n, ld, seed, kind)
         if check:
@@ -302,6 +383,11 @@ def tail_mode_name(v):
 
 def trsm_panel_name(v):
     s = load().rtat_trsm_panel_name(v)
+    return s.decode() if s is not None else None
+
+
+def activation_name(v):
+    s = load().rtat_activation_name(v)
     return s.decode() if s is not None else None
 
 
