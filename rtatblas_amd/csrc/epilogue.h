@@ -25,6 +25,9 @@ template <> struct Half<__bf16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec_t, a),
                                                    __builtin_bit_cast(vec_t, b), c, 0, 0, 0);
   }
+  __device__ static inline void mfma_into(f4_t& c, s8_t a, s8_t b) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  }
 };
 template <> struct Half<_Float16> {
   typedef f16x8_t vec_t;
@@ -33,7 +36,19 @@ template <> struct Half<_Float16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec_t, a),
                                                   __builtin_bit_cast(vec_t, b), c, 0, 0, 0);
   }
+  __device__ static inline void mfma_into(f4_t& c, s8_t a, s8_t b) {
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  }
 };
+// mfma_into keeps the accumulator in the accumulation registers and its place in the program: a
+// wave that holds 256 of them leaves the compiler no room to move them about, which it otherwise
+// does every iteration.  The compiler does not see a matrix instruction there, so nothing but
+// mfma_into may touch the accumulators until mfma_settle has passed.
+__device__ inline void mfma_settle() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
 
 // Sixteen bytes at an address that is only element-aligned (one global load: the hardware
 // accepts any alignment).

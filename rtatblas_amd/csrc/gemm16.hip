@@ -71,32 +71,38 @@ struct Panel16 {
   }
 };
 
-// Fragments of MFMA K-step `step` (0 or 1) for TB blocks of 16 rows starting at row w0.
-template <bool KMAJOR, int ROWS, int TB>
-__device__ inline void read_frags(const unsigned char* panel, int w0, int step, int lane,
-                                  s8_t (&f)[TB]) {
+// This lane's place in the MFMA operands of a panel whose wave tile starts at row w0 (a multiple
+// of 16): operand `block` (16 rows) of K-step `step` (0 or 1).
+template <bool KMAJOR, int ROWS>
+struct Frags16 {
   typedef Panel16<KMAJOR, ROWS> P;
-  const int l16 = lane & 15, q = lane >> 4;
-  if constexpr (KMAJOR) {
-    const int chunk = (4 * step + q) ^ P::key(l16);
-    const unsigned char* at = panel + (w0 + l16) * P::ROWBYTES + chunk * 16;
-#pragma unroll
-    for (int b = 0; b < TB; ++b) f[b] = *reinterpret_cast<const s8_t*>(at + b * 16 * P::ROWBYTES);
-  } else {
-    typedef __attribute__((address_space(3))) s4_t* lds4_t;
-    // Lane j of a group addresses 4 elements at row k = 8 q + j / 4 (and + 4), column 4 (j % 4).
-    const int k = 32 * step + 8 * q + (l16 >> 2), key = P::key(k & 15);
-    const unsigned char* row = panel + k * P::ROWBYTES + (l16 & 1) * 8;
-#pragma unroll
-    for (int b = 0; b < TB; ++b) {
-      const int chunk = (w0 / 8 + 2 * b + ((l16 >> 1) & 1)) ^ key;
-      const unsigned char* at = row + chunk * 16;
-      const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(at));
-      const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(at + 4 * P::ROWBYTES));
-      f[b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  int base;  // bytes
+  int flip;  // what the chunk number is XORed with, times 16
+  __device__ inline Frags16(int w0, int lane) {
+    const int l16 = lane & 15, q = lane >> 4;
+    if constexpr (KMAJOR) {
+      base = (w0 + l16) * P::ROWBYTES;
+      flip = (q ^ P::key(l16)) * 16;
+    } else {
+      // Lane j of a group addresses 4 elements at row k = 8 q + j / 4 (and + 4), column 4 (j % 4).
+      const int k = 8 * q + (l16 >> 2);
+      base = k * P::ROWBYTES + (l16 & 1) * 8;
+      flip = ((w0 / 8 + ((l16 >> 1) & 1)) ^ P::key(k & 15)) * 16;
     }
   }
-}
+  __device__ inline s8_t read(const unsigned char* panel, int block, int step) const {
+    if constexpr (KMAJOR) {
+      return *reinterpret_cast<const s8_t*>(panel + base + (flip ^ (step * 64)) +
+                                            block * 16 * P::ROWBYTES);
+    } else {
+      typedef __attribute__((address_space(3))) s4_t* lds4_t;
+      const unsigned char* at = panel + base + step * 32 * P::ROWBYTES + (flip ^ (block * 32));
+      const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(at));
+      const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(at + 4 * P::ROWBYTES));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
 
 // Global -> register -> LDS mover of one panel: any alignment, leading dimension and edge.
 // Rows past row_lim repeat the last one (they reach accumulators that are not stored), k past
@@ -141,65 +147,15 @@ struct Mover16 {
   }
 };
 
-template <class T, class S, bool KA, bool KB>
-__global__ __launch_bounds__(S::NT, S::OCC) void gemm16_kernel(Gemm16Args p) {
+// The epilogue of a tile, a block column (16 columns of C) at a time: the wave parks it in its own
+// part of LDS, column by column, and takes it back as eight neighbouring rows per lane.
+template <class S>
+__device__ inline void finish_tile(const Gemm16Args& p, unsigned char* lds, int tile_m, int tile_n,
+                                   long z, int wave, int lane,
+                                   const f4_t (&acc)[S::TM][S::TN]) {
   constexpr int TM = S::TM, TN = S::TN;
-  extern __shared__ __align__(16) unsigned char lds[];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int wm0 = (wave % S::WGM) * S::WTM, wn0 = (wave / S::WGM) * S::WTN;
-
-  const int logical = logical_of_workgroup(blockIdx.x, gridDim.x);
-  const long z = logical / p.tiles;
-  int tile_m, tile_n;
-  tile_of_logical(logical % p.tiles, p.tiles_m, p.tiles_n, p.tri, S::BM, S::BN, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::BN;
-  const uint16_t* A = p.A + z * p.a_stride;
-  const uint16_t* B = p.B + z * p.b_stride;
-
-  f4_t acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{0, 0, 0, 0};
-
-  const int panels = (p.k + BK16 - 1) / BK16;
-  typedef Panel16<KA, S::BM> PA;
-  Mover16<KA, S::BM, S::NT> ma;
-  Mover16<KB, S::BN, S::NT> mb;
-  auto load = [&](int kt) {
-    ma.load(A, p.lda, m0, p.m, kt * BK16, p.k, t);
-    mb.load(B, p.ldb, n0, p.n, kt * BK16, p.k, t);
-  };
-  auto store = [&](int kt) {
-    unsigned char* stage = lds + (kt & 1) * S::STAGE;
-    ma.store(stage, t);
-    mb.store(stage + PA::BYTES, t);
-  };
-  if (panels > 0) {
-    load(0);
-    store(0);
-    if (panels > 1) load(1);
-  }
-  __syncthreads();
-  for (int kt = 0; kt < panels; ++kt) {
-    const unsigned char* stage = lds + (kt & 1) * S::STAGE;
-    if (kt + 1 < panels) store(kt + 1);
-    if (kt + 2 < panels) load(kt + 2);
-#pragma unroll
-    for (int step = 0; step < 2; ++step) {
-      s8_t fa[TM], fb[TN];
-      read_frags<KA, S::BM>(stage, wm0, step, lane, fa);
-      read_frags<KB, S::BN>(stage + PA::BYTES, wn0, step, lane, fb);
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = Half<T>::mfma(fa[i], fb[j], acc[i][j]);
-    }
-    __syncthreads();
-  }
-
-  // Epilogue, a block column (16 columns of C) at a time: the wave parks it in its own part of
-  // LDS, column by column, and takes it back as eight neighbouring rows per lane.
+  const int wm0 = (wave % S::WGM) * S::WTM, wn0 = (wave / S::WGM) * S::WTN;
   const Epilogue& e = p.ep;
   float alpha = e.alpha, beta = e.beta;
   int c_exp = 0;
@@ -270,13 +226,252 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_kernel(Gemm16Args p) {
   }
 }
 
+template <class T, class S, bool KA, bool KB>
+__global__ __launch_bounds__(S::NT, S::OCC) void gemm16_kernel(Gemm16Args p) {
+  constexpr int TM = S::TM, TN = S::TN;
+  extern __shared__ __align__(16) unsigned char lds[];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int wm0 = (wave % S::WGM) * S::WTM, wn0 = (wave / S::WGM) * S::WTN;
+
+  const int logical = logical_of_workgroup(blockIdx.x, gridDim.x);
+  const long z = logical / p.tiles;
+  int tile_m, tile_n;
+  tile_of_logical(logical % p.tiles, p.tiles_m, p.tiles_n, p.tri, S::BM, S::BN, tile_m, tile_n);
+  const int m0 = tile_m * S::BM, n0 = tile_n * S::BN;
+  const uint16_t* A = p.A + z * p.a_stride;
+  const uint16_t* B = p.B + z * p.b_stride;
+
+  f4_t acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{0, 0, 0, 0};
+
+  const int panels = (p.k + BK16 - 1) / BK16;
+  typedef Panel16<KA, S::BM> PA;
+  const Frags16<KA, S::BM> ra(wm0, lane);
+  const Frags16<KB, S::BN> rb(wn0, lane);
+  Mover16<KA, S::BM, S::NT> ma;
+  Mover16<KB, S::BN, S::NT> mb;
+  auto load = [&](int kt) {
+    ma.load(A, p.lda, m0, p.m, kt * BK16, p.k, t);
+    mb.load(B, p.ldb, n0, p.n, kt * BK16, p.k, t);
+  };
+  auto store = [&](int kt) {
+    unsigned char* stage = lds + (kt & 1) * S::STAGE;
+    ma.store(stage, t);
+    mb.store(stage + PA::BYTES, t);
+  };
+  if (panels > 0) {
+    load(0);
+    store(0);
+    if (panels > 1) load(1);
+  }
+  __syncthreads();
+  for (int kt = 0; kt < panels; ++kt) {
+    const unsigned char* stage = lds + (kt & 1) * S::STAGE;
+    if (kt + 1 < panels) store(kt + 1);
+    if (kt + 2 < panels) load(kt + 2);
+#pragma unroll
+    for (int step = 0; step < 2; ++step) {
+      s8_t fa[TM], fb[TN];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) fa[i] = ra.read(stage, i, step);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fb[j] = rb.read(stage + PA::BYTES, j, step);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = Half<T>::mfma(fa[i], fb[j], acc[i][j]);
+    }
+    __syncthreads();
+  }
+  finish_tile<S>(p, lds, tile_m, tile_n, z, wave, lane, acc);
+}
+
+// Global -> LDS mover of one whole panel (buffer loads that write LDS): nothing passes through
+// registers.  Needs 16-byte aligned columns and every k in range; rows over the edge repeat the
+// last row (k-major) or the last chunk that starts inside (mn-major: such a chunk may run into
+// the next column, so the panel that holds an operand's last column takes Mover16 instead).
+template <bool KMAJOR, int ROWS, int NW>
+struct Dma16 {
+  typedef Panel16<KMAJOR, ROWS> P;
+  static constexpr int NI = P::BYTES / (1024 * NW);
+  unsigned off[NI];  // bytes from the panel's first element in memory
+
+  __device__ inline void init(long ld, int row0, int row_lim, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = (i * NW + wave) * 64 + lane, lr = c / P::CHUNKS, e0 = P::source_chunk(c) * 8;
+      if constexpr (KMAJOR) {
+        const int row = row0 + lr < row_lim ? lr : row_lim - 1 - row0;
+        off[i] = (unsigned)(((long)row * ld + e0) * 2);
+      } else {
+        const int last = ((row_lim - 1) & ~7) - row0;
+        off[i] = (unsigned)(((long)lr * ld + (e0 < last ? e0 : last)) * 2);
+      }
+    }
+  }
+  // Instruction i of a panel (`where`: panel_at).  Written in assembly because behind the builtin
+  // the compiler waits for every load in flight before each transposing LDS read (the s_nop is the
+  // wait state between M0 and a load to LDS); it has no
+  // result register, and wait_all_and_meet is its wait; nothing else here reads M0.
+  __device__ inline void issue(int i, u4_t where, unsigned panel, int wave) const {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(panel + (unsigned)(i * NW + wave) * 1024u), "v"(off[i]), "s"(where));
+  }
+  // Buffer descriptor of panel kt of the operand whose first element of the tile is `base`.
+  __device__ static inline u4_t panel_at(const uint16_t* base, long ld, int kt) {
+    const uint64_t at =
+        reinterpret_cast<uint64_t>(base + (KMAJOR ? (long)kt * BK16 : (long)kt * BK16 * ld));
+    return u4_t{(unsigned)at, (unsigned)(at >> 32) & 0xffffu, 0xffffffffu, 0x00020000u};
+  }
+};
+__device__ inline unsigned lds_address(const unsigned char* p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p;
+}
+
+// Everything this wave asked for has arrived and everything it read is in registers; then the
+// same of all waves.
+[[maybe_unused]] __device__ inline void wait_all_and_meet() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The large-tile kernel: 256 x 256 by four waves of 128 x 128, one workgroup per CU.
+//   * A wave holds 128 x 128 of C in 256 accumulator registers, which needs the fewest LDS bytes
+//     per MFMA (32 reads of 1 KiB for 128 MFMAs of 16 clocks; eight waves of 128 x 64 would ask LDS
+//     for 48 in the time it delivers 48).
+//   * Panel kt + 2 is on its way into the stage that panel kt just left while panel kt + 1 is
+//     computed: loads go straight to LDS, so they cost no registers.  One barrier per panel, half
+//     way through it: by then the second half's operands are in registers, so the stage is free,
+//     and the next panel, asked for one panel ago, has arrived.
+//   * Within a half the LDS reads of the next half and the panel loads are spread behind the
+//     MFMAs one by one.
+template <class T, class S, bool KA, bool KB>
+__global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p) {
+#if defined(__HIP_DEVICE_COMPILE__)  // the host pass wants the launch stub only
+  constexpr int TM = S::TM, TN = S::TN;
+  extern __shared__ __align__(16) unsigned char lds[];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int wm0 = (wave % S::WGM) * S::WTM, wn0 = (wave / S::WGM) * S::WTN;
+
+  const int logical = logical_of_workgroup(blockIdx.x, gridDim.x);
+  const long z = logical / p.tiles;
+  int tile_m, tile_n;
+  tile_of_logical(logical % p.tiles, p.tiles_m, p.tiles_n, p.tri, S::BM, S::BN, tile_m, tile_n);
+  const int m0 = tile_m * S::BM, n0 = tile_n * S::BN;
+  const uint16_t* A = p.A + z * p.a_stride;
+  const uint16_t* B = p.B + z * p.b_stride;
+  const uint16_t* At = A + (KA ? (long)m0 * p.lda : (long)m0);
+  const uint16_t* Bt = B + (KB ? (long)n0 * p.ldb : (long)n0);
+
+  f4_t acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{0, 0, 0, 0};
+
+  typedef Panel16<KA, S::BM> PA;
+  Dma16<KA, S::BM, S::NW> da;
+  Dma16<KB, S::BN, S::NW> db;
+  da.init(p.lda, m0, p.m, wave, lane);
+  db.init(p.ldb, n0, p.n, wave, lane);
+  // Panels 0 .. whole - 1 go straight to LDS; a last one may need guards.
+  const int panels = (p.k + BK16 - 1) / BK16;
+  const bool ragged = p.k % BK16 != 0 || (!KA && m0 + S::BM > p.m) || (!KB && n0 + S::BN > p.n);
+  const int whole = panels - (ragged ? 1 : 0);
+  auto issue_all = [&](int kt) {
+    unsigned char* stage = lds + (kt & 1) * S::STAGE;
+    if (kt < whole) {
+      const u4_t pa = da.panel_at(At, p.lda, kt), pb = db.panel_at(Bt, p.ldb, kt);
+      const unsigned to = lds_address(stage);
+#pragma unroll
+      for (int i = 0; i < da.NI; ++i) da.issue(i, pa, to, wave);
+#pragma unroll
+      for (int i = 0; i < db.NI; ++i) db.issue(i, pb, to + PA::BYTES, wave);
+    } else {
+      {
+        Mover16<KA, S::BM, S::NT> ma;
+        ma.load(A, p.lda, m0, p.m, kt * BK16, p.k, t);
+        ma.store(stage, t);
+      }
+      Mover16<KB, S::BN, S::NT> mb;
+      mb.load(B, p.ldb, n0, p.n, kt * BK16, p.k, t);
+      mb.store(stage + PA::BYTES, t);
+    }
+  };
+
+  const Frags16<KA, S::BM> ra(wm0, lane);
+  const Frags16<KB, S::BN> rb(wn0, lane);
+  s8_t fa[2][TM], fb[2][TN];
+  // Operand x of a K-step, in the order the MFMAs want them: the first row of A, B, the other rows.
+  auto read = [&](int stage, int step, int x) {
+    const unsigned char* at = lds + stage * S::STAGE;
+    if (x == 0 || x > TN) fa[step][x == 0 ? 0 : x - TN] = ra.read(at, x == 0 ? 0 : x - TN, step);
+    else fb[step][x - 1] = rb.read(at + PA::BYTES, x - 1, step);
+  };
+  // The MFMAs of one K-step with `side(x)`, x = 0 .. TM + TN - 1, spread behind the first three
+  // quarters of them.
+  auto multiply = [&](int step, auto side) {
+    constexpr int GAP = 3 * TM * TN / (4 * (TM + TN));
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int x = i * TN + j;
+        Half<T>::mfma_into(acc[i][j], fa[step][i], fb[step][j]);
+        if (x % GAP == 0 && x / GAP < TM + TN) {
+          side(x / GAP);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+  };
+  static_assert(TM + TN == decltype(da)::NI + decltype(db)::NI, "a load goes with every LDS read");
+
+  if (panels > 0) {
+    issue_all(0);
+    wait_all_and_meet();
+    if (panels > 1) issue_all(1);
+#pragma unroll
+    for (int x = 0; x < TM + TN; ++x) read(0, 0, x);
+  }
+  int kt = 0;
+  for (; kt < whole - 2; ++kt) {
+    const int cur = kt & 1, nxt = cur ^ 1;
+    multiply(0, [&](int x) { read(cur, 1, x); });
+    wait_all_and_meet();
+    const unsigned to = lds_address(lds + cur * S::STAGE);
+    const u4_t pa = da.panel_at(At, p.lda, kt + 2), pb = db.panel_at(Bt, p.ldb, kt + 2);
+    multiply(1, [&](int x) {
+      if (x < da.NI) da.issue(x, pa, to, wave);
+      else db.issue(x - da.NI, pb, to + PA::BYTES, wave);
+      read(nxt, 0, x);
+    });
+  }
+#pragma unroll 1
+  for (; kt < panels; ++kt) {
+    const int cur = kt & 1, nxt = cur ^ 1;
+    multiply(0, [&](int x) { read(cur, 1, x); });
+    wait_all_and_meet();
+    if (kt + 2 < panels) issue_all(kt + 2);
+    multiply(1, [&](int x) { read(nxt, 0, x); });  // of the last panel: not used
+  }
+  mfma_settle();
+  __syncthreads();
+  finish_tile<S>(p, lds, tile_m, tile_n, z, wave, lane, acc);
+#endif
+}
+
+typedef Shape16<256, 256, 2, 2, 1> S256x256;  // loads straight to LDS
 typedef Shape16<128, 128, 2, 2, 2> S128x128;
 typedef Shape16<64, 64, 2, 2, 4> S64x64;
 
-template <class T, class S, bool KA, bool KB>
-rtat_status_t launch_shape(rtat_native_handle* h, const Gemm16& g, Gemm16Args p) {
-  static PerDeviceOnce configured;
-  auto kern = gemm16_kernel<T, S, KA, KB>;
+template <class S>
+rtat_status_t launch_kernel(rtat_native_handle* h, const Gemm16& g, Gemm16Args p,
+                            void (*kern)(Gemm16Args), PerDeviceOnce& configured) {
   if (!configured(h->device, [&] {
         if (S::LDS <= 65536) return true;
         if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
@@ -296,21 +491,40 @@ rtat_status_t launch_shape(rtat_native_handle* h, const Gemm16& g, Gemm16Args p)
   return launch_status();
 }
 
-template <class T, class S>
+template <class T, class S, bool KA, bool KB, bool DMA>
+rtat_status_t launch_shape(rtat_native_handle* h, const Gemm16& g, const Gemm16Args& p) {
+  static PerDeviceOnce configured;
+  if constexpr (DMA) return launch_kernel<S>(h, g, p, &gemm16_dma_kernel<T, S, KA, KB>, configured);
+  else return launch_kernel<S>(h, g, p, &gemm16_kernel<T, S, KA, KB>, configured);
+}
+
+template <class T, class S, bool DMA>
 rtat_status_t launch_ops16(rtat_native_handle* h, const Gemm16& g, const Gemm16Args& p) {
   const bool ka = g.ta, kb = !g.tb;  // contiguous along k
-  if (ka && kb) return launch_shape<T, S, true, true>(h, g, p);
-  if (ka) return launch_shape<T, S, true, false>(h, g, p);
-  if (kb) return launch_shape<T, S, false, true>(h, g, p);
-  return launch_shape<T, S, false, false>(h, g, p);
+  if (ka && kb) return launch_shape<T, S, true, true, DMA>(h, g, p);
+  if (ka) return launch_shape<T, S, true, false, DMA>(h, g, p);
+  if (kb) return launch_shape<T, S, false, true, DMA>(h, g, p);
+  return launch_shape<T, S, false, false, DMA>(h, g, p);
+}
+
+// Whether panels of an operand may go straight to LDS: 16-byte aligned columns, and the farthest
+// element of a 256-row panel within 32-bit byte offsets.
+bool direct(const void* base, long ld, long stride) {
+  return ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(ld * 2) | (uintptr_t)(stride * 2)) & 15) == 0 &&
+         ld < (1L << 23);
 }
 
 template <class T>
 rtat_status_t launch_type(rtat_native_handle* h, const Gemm16& g, const Gemm16Args& p) {
   const long cus = h->compute_units > 0 ? h->compute_units : 256;
-  const long big = (long)((p.m + 127) / 128) * ((p.n + 127) / 128) * g.batch / (p.tri ? 2 : 1);
-  if (big >= cus) return launch_ops16<T, S128x128>(h, g, p);
-  return launch_ops16<T, S64x64>(h, g, p);
+  auto tiles = [&](int b) {
+    return (long)((p.m + b - 1) / b) * ((p.n + b - 1) / b) * g.batch / (p.tri ? 2 : 1);
+  };
+  if (direct(p.A, p.lda, p.a_stride) && direct(p.B, p.ldb, p.b_stride)) {
+    if (tiles(256) >= cus / 2) return launch_ops16<T, S256x256, true>(h, g, p);
+  }
+  if (tiles(128) >= cus) return launch_ops16<T, S128x128, false>(h, g, p);
+  return launch_ops16<T, S64x64, false>(h, g, p);
 }
 
 __global__ __launch_bounds__(256) void sum_rows_kernel(const float* parts, int count, int m,
