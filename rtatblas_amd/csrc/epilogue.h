@@ -139,7 +139,13 @@ __device__ inline void store_one(int type, void* p, long i, float x) {
   else static_cast<uint16_t*>(p)[i] = float_to_half(type, x);
 }
 
-// Eight neighbours on a 16-byte boundary.
+// Eight neighbours, at any element-aligned address.
+__device__ inline u4_t load16(const void* p, long byte) {
+  return reinterpret_cast<const Loose16*>(static_cast<const char*>(p) + byte)->v;
+}
+__device__ inline void store16(void* p, long byte, u4_t v) {
+  reinterpret_cast<Loose16*>(static_cast<char*>(p) + byte)->v = v;
+}
 __device__ inline void unpack8(int type, u4_t raw, float (&v)[8]) {
   if (type == RTAT_TYPE_BF16) {
     const bf16x8_t h = __builtin_bit_cast(bf16x8_t, raw);
@@ -163,33 +169,73 @@ __device__ inline u4_t pack8(int type, const float (&v)[8]) {
   for (int e = 0; e < 8; ++e) h[e] = (_Float16)v[e];
   return __builtin_bit_cast(u4_t, h);
 }
-__device__ inline void load8(int type, const void* p, long i, float (&v)[8]) {
+// The bits of eight elements from element i on; `hi` only for F32.
+struct Raw8 {
+  u4_t lo, hi;
+};
+__device__ inline Raw8 fetch8(int type, const void* p, long i) {
+  Raw8 r = {};
   if (type == RTAT_TYPE_F32) {
-    const f4_t* q = reinterpret_cast<const f4_t*>(static_cast<const float*>(p) + i);
-    const f4_t a = q[0], b = q[1];
+    r.lo = load16(p, 4 * i);
+    r.hi = load16(p, 4 * i + 16);
+  } else {
+    r.lo = load16(p, 2 * i);
+  }
+  return r;
+}
+__device__ inline void unpack8(int type, const Raw8& r, float (&v)[8]) {
+  if (type == RTAT_TYPE_F32) {
+    const f4_t a = __builtin_bit_cast(f4_t, r.lo), b = __builtin_bit_cast(f4_t, r.hi);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[e] = a[e];
       v[4 + e] = b[e];
     }
   } else {
-    unpack8(type, *reinterpret_cast<const u4_t*>(static_cast<const uint16_t*>(p) + i), v);
+    unpack8(type, r.lo, v);
   }
+}
+__device__ inline void load8(int type, const void* p, long i, float (&v)[8]) {
+  unpack8(type, fetch8(type, p, i), v);
 }
 __device__ inline void store8(int type, void* p, long i, const float (&v)[8]) {
   if (type == RTAT_TYPE_F32) {
-    f4_t* q = reinterpret_cast<f4_t*>(static_cast<float*>(p) + i);
-    f4_t a, b;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      a[e] = v[e];
-      b[e] = v[4 + e];
-    }
-    q[0] = a;
-    q[1] = b;
+    store16(p, 4 * i, __builtin_bit_cast(u4_t, f4_t{v[0], v[1], v[2], v[3]}));
+    store16(p, 4 * i + 16, __builtin_bit_cast(u4_t, f4_t{v[4], v[5], v[6], v[7]}));
   } else {
-    *reinterpret_cast<u4_t*>(static_cast<uint16_t*>(p) + i) = pack8(type, v);
+    store16(p, 2 * i, pack8(type, v));
   }
+}
+
+// Eight elements through an activation; the choice is made once for all of them.
+__device__ inline void act_values(int act, float (&v)[8]) {
+#define RTAT_EACH(A)                                                    \
+  case A:                                                               \
+    _Pragma("unroll") for (int i = 0; i < 8; ++i) v[i] = act_value(A, v[i]); \
+    break;
+  switch (act) {
+    RTAT_EACH(RTAT_ACT_RELU)
+    RTAT_EACH(RTAT_ACT_GELU)
+    RTAT_EACH(RTAT_ACT_GELU_TANH)
+    RTAT_EACH(RTAT_ACT_SILU)
+    default: break;
+  }
+#undef RTAT_EACH
+}
+// v *= act'(z)
+__device__ inline void act_slopes(int act, const float (&z)[8], float (&v)[8]) {
+#define RTAT_EACH(A)                                                          \
+  case A:                                                                     \
+    _Pragma("unroll") for (int i = 0; i < 8; ++i) v[i] *= act_slope(A, z[i]); \
+    break;
+  switch (act) {
+    RTAT_EACH(RTAT_ACT_RELU)
+    RTAT_EACH(RTAT_ACT_GELU)
+    RTAT_EACH(RTAT_ACT_GELU_TANH)
+    RTAT_EACH(RTAT_ACT_SILU)
+    default: break;
+  }
+#undef RTAT_EACH
 }
 
 // What becomes of the product.  Elements (row, col) with row < rows and col < cols are stored.
@@ -218,20 +264,7 @@ struct Epilogue {
   float* sums;  // gradient: one row of `rows` partial sums per wave column of the launch
   const float* scale;
   int r_power, scale_c;
-  int vec;  // 1: bias, aux, C and D may be accessed sixteen bytes at a time at rows 8 i
 };
-
-// Sixteen-byte access at rows that are multiples of eight: base and column stride in bytes
-// (and the batch's) are multiples of 16.
-inline bool vec_ok(const void* p, long ld, long stride, int type) {
-  const long es = type_bytes(type);
-  return p == nullptr || ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * es) | (uintptr_t)(stride * es)) & 15) == 0;
-}
-inline void settle_vec(Epilogue& e) {
-  e.vec = vec_ok(e.bias, 0, 0, e.bias_type) && vec_ok(e.aux, e.ldaux, e.aux_stride, e.aux_type) &&
-          vec_ok(e.C, e.ldc, e.c_stride, e.c_type) &&
-          vec_ok(e.copy, e.ldcopy, e.copy_stride, RTAT_TYPE_F16) && vec_ok(e.D, e.ldd, e.d_stride, e.d_type);
-}
 
 // Rows row .. row + 7 of column col, batch matrix z: v holds the accumulators and, for a
 // gradient, leaves with the values that belong to the row sums (0 outside).
@@ -247,13 +280,12 @@ __device__ inline void epilogue8(const Epilogue& e, float alpha, float beta, int
   const long c_at = z * e.c_stride + row + (long)col * e.ldc;
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] *= alpha;
-  if (e.vec && row + 8 <= e.rows && (e.C == nullptr || row + 8 <= e.c_rows)) {
+  if (row + 8 <= e.rows && (e.C == nullptr || row + 8 <= e.c_rows)) {
     float w[8];
     if (e.slope) {
       if (e.act != RTAT_ACT_NONE) {
         load8(e.aux_type, e.aux, aux_at, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= act_slope(e.act, w[i]);
+        act_slopes(e.act, w, v);
       }
     } else {
       float c[8];
@@ -265,14 +297,10 @@ __device__ inline void epilogue8(const Epilogue& e, float alpha, float beta, int
         for (int i = 0; i < 8; ++i) v[i] += w[i];
       }
       if (e.aux != nullptr) store8(e.aux_type, e.aux, aux_at, v);
-      if (e.act != RTAT_ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = act_value(e.act, v[i]);
-      }
+      act_values(e.act, v);
       if (with_c) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          v[i] = __builtin_fmaf(beta, c_exp ? __builtin_ldexpf(c[i], c_exp) : c[i], v[i]);
+        for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(beta, __builtin_ldexpf(c[i], c_exp), v[i]);
       }
     }
     store8(e.d_type, e.D, d_at, v);

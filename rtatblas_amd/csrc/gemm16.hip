@@ -150,13 +150,125 @@ struct Mover16 {
 // The epilogue of a tile, a block column (16 columns of C) at a time: the wave parks it in its own
 // part of LDS, column by column, and takes it back as eight neighbouring rows per lane.
 template <class S>
-__device__ inline void finish_tile(const Gemm16Args& p, unsigned char* lds, int tile_m, int tile_n,
+struct Parked {
+  static constexpr int LPC = S::WTM / 8;   // lanes per column
+  static constexpr int CPP = 64 / LPC;     // columns per pass
+  static constexpr int PASSES = 16 / CPP;  // passes per block column
+  float* park;
+  int lane, row, col;  // this lane's first row of the wave tile, its column within a pass
+
+  __device__ inline Parked(unsigned char* lds, int wave, int lane_)
+      : park(reinterpret_cast<float*>(lds) + wave * 16 * S::PARK), lane(lane_),
+        row((lane_ % LPC) * 8), col(lane_ / LPC) {}
+  // Between a wave's writes and its own reads of what other lanes wrote: LDS keeps the order of a
+  // wave's accesses, the compiler has to be told.
+  __device__ static inline void turn() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  // Block column j, J <= j < TN: the accumulators must be named by constants.
+  template <int J = 0>
+  __device__ __forceinline__ void put(int j, const f4_t (&acc)[S::TM][S::TN]) const {
+    if (j == J) {
+      turn();
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i)
+        *reinterpret_cast<f4_t*>(park + (lane & 15) * S::PARK + 16 * i + 4 * (lane >> 4)) = acc[i][J];
+      turn();
+    } else if constexpr (J + 1 < S::TN) {
+      put<J + 1>(j, acc);
+    }
+  }
+  __device__ inline void get(int pass, float (&v)[8]) const {
+    const f4_t* at = reinterpret_cast<const f4_t*>(park + (pass * CPP + col) * S::PARK + row);
+    const f4_t lo = at[0], hi = at[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = lo[i];
+      v[4 + i] = hi[i];
+    }
+  }
+  // The block column as rows of the mirrored tile: lane pairs take its two halves.
+  __device__ inline void get_mirrored(int r0, float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = park[(8 * (lane & 1) + i) * S::PARK + r0 + (lane >> 1)];
+  }
+};
+
+// A tile that lies wholly inside C: nothing to check, and what a block column needs from memory
+// (the residual, or the argument of the activation) is asked for one block column ahead.
+template <class S, bool SLOPE>
+__device__ __forceinline__ void finish_inside(const Epilogue& e, const Parked<S>& k, float alpha, float beta,
+                                     int c_exp, int m0, int n0, long z,
+                                     const f4_t (&acc)[S::TM][S::TN], float (&sums)[8]) {
+  constexpr int PASSES = Parked<S>::PASSES;
+  const int row = m0 + k.row, col = n0 + k.col;
+  const void* in = SLOPE ? (e.act != RTAT_ACT_NONE ? e.aux : nullptr) : e.C;
+  const int in_type = SLOPE ? e.aux_type : e.c_type;
+  const long ldin = SLOPE ? e.ldaux : e.ldc;
+  const long in0 = z * (SLOPE ? e.aux_stride : e.c_stride) + row + col * ldin;
+  const long d0 = z * e.d_stride + row + col * e.ldd;
+  const long aux0 = z * e.aux_stride + row + col * e.ldaux;
+  const long copy0 = z * e.copy_stride + row + col * e.ldcopy;
+  float bias[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bias[i] = 0.0f;
+  if (!SLOPE && e.bias != nullptr) load8(e.bias_type, e.bias, row, bias);
+  Raw8 next[PASSES];
+  auto ask = [&](int j) {
+    if (in != nullptr) {
+#pragma unroll
+      for (int q = 0; q < PASSES; ++q)
+        next[q] = fetch8(in_type, in, in0 + (16 * j + q * Parked<S>::CPP) * ldin);
+    }
+  };
+  ask(0);
+#pragma unroll 1
+  for (int j = 0; j < S::TN; ++j) {
+    k.put(j, acc);
+    Raw8 now[PASSES];
+#pragma unroll
+    for (int q = 0; q < PASSES; ++q) now[q] = next[q];
+    if (j + 1 < S::TN) ask(j + 1);
+    float v[PASSES][8];
+#pragma unroll
+    for (int q = 0; q < PASSES; ++q) k.get(q, v[q]);
+#pragma unroll
+    for (int q = 0; q < PASSES; ++q) {
+      const long c = 16 * j + q * Parked<S>::CPP;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[q][i] = __builtin_fmaf(v[q][i], alpha, bias[i]);
+      float w[8];
+      if (in != nullptr) unpack8(in_type, now[q], w);
+      if constexpr (SLOPE) {
+        if (in != nullptr) act_slopes(e.act, w, v[q]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sums[i] += v[q][i];
+      } else {
+        if (e.aux != nullptr) store8(e.aux_type, e.aux, aux0 + c * e.ldaux, v[q]);
+        act_values(e.act, v[q]);
+        if (in != nullptr) {
+          if (c_exp != 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __builtin_ldexpf(w[i], c_exp);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[q][i] = __builtin_fmaf(beta, w[i], v[q][i]);
+        }
+      }
+      store8(e.d_type, e.D, d0 + c * e.ldd, v[q]);
+      if (!SLOPE && e.copy != nullptr) store8(RTAT_TYPE_F16, e.copy, copy0 + c * e.ldcopy, v[q]);
+    }
+  }
+}
+
+template <class S>
+__device__ __forceinline__ void finish_tile(const Gemm16Args& p, unsigned char* lds, int tile_m, int tile_n,
                                    long z, int wave, int lane,
                                    const f4_t (&acc)[S::TM][S::TN]) {
-  constexpr int TM = S::TM, TN = S::TN;
-  const int m0 = tile_m * S::BM, n0 = tile_n * S::BN;
-  const int wm0 = (wave % S::WGM) * S::WTM, wn0 = (wave / S::WGM) * S::WTN;
   const Epilogue& e = p.ep;
+  const int m0 = tile_m * S::BM + (wave % S::WGM) * S::WTM;  // of the wave tile
+  const int n0 = tile_n * S::BN + (wave / S::WGM) * S::WTN;
   float alpha = e.alpha, beta = e.beta;
   int c_exp = 0;
   if (e.scale != nullptr) {
@@ -167,52 +279,41 @@ __device__ inline void finish_tile(const Gemm16Args& p, unsigned char* lds, int 
       c_exp = (int)e.scale[2 * z + 1];
     }
   }
-  float* park = reinterpret_cast<float*>(lds) + wave * 16 * S::PARK;
-  constexpr int LPC = S::WTM / 8;   // lanes per column
-  constexpr int CPP = 64 / LPC;     // columns per pass
-  const int er = (lane % LPC) * 8;  // row of this lane inside the wave tile
+  const Parked<S> k(lds, wave, lane);
   float sums[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) sums[i] = 0.0f;
   const bool mirror = p.tri != 0 && tile_m != tile_n;
+  const bool inside = m0 + S::WTM <= e.rows && n0 + S::WTN <= e.cols &&
+                      (e.C == nullptr || (m0 + S::WTM <= e.c_rows && n0 + S::WTN <= e.c_cols));
+  if (inside && !mirror) {
+    if (e.slope) finish_inside<S, true>(e, k, alpha, beta, c_exp, m0, n0, z, acc, sums);
+    else finish_inside<S, false>(e, k, alpha, beta, c_exp, m0, n0, z, acc, sums);
+  } else {
 #pragma unroll 1
-  for (int j = 0; j < TN; ++j) {
-#pragma unroll
-    for (int jj = 0; jj < TN; ++jj)
-      if (jj == j) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-          *reinterpret_cast<f4_t*>(park + (lane & 15) * S::PARK + 16 * i + 4 * (lane >> 4)) =
-              acc[i][jj];
-      }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    for (int j = 0; j < S::TN; ++j) {
+      k.put(j, acc);
 #pragma unroll 1
-    for (int c0 = 0; c0 < 16; c0 += CPP) {
-      const int c = c0 + lane / LPC;
-      const f4_t* at = reinterpret_cast<const f4_t*>(park + c * S::PARK + er);
-      const f4_t lo = at[0], hi = at[1];
-      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      epilogue8(e, alpha, beta, c_exp, m0 + wm0 + er, n0 + wn0 + 16 * j + c, z, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sums[i] += v[i];
-    }
-    if (mirror) {
-      // The same 16 columns as rows of the mirrored tile: lane pairs take the two halves.
-#pragma unroll 1
-      for (int r0 = 0; r0 < S::WTM; r0 += 32) {
-        const int r = r0 + (lane >> 1), c = 8 * (lane & 1);
+      for (int q = 0; q < Parked<S>::PASSES; ++q) {
         float v[8];
+        k.get(q, v);
+        epilogue8(e, alpha, beta, c_exp, m0 + k.row, n0 + 16 * j + q * Parked<S>::CPP + k.col, z, v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = park[(c + i) * S::PARK + r];
-        epilogue8(e, alpha, beta, c_exp, n0 + wn0 + 16 * j + c, m0 + wm0 + r, z, v);
+        for (int i = 0; i < 8; ++i) sums[i] += v[i];
+      }
+      if (mirror) {
+#pragma unroll 1
+        for (int r0 = 0; r0 < S::WTM; r0 += 32) {
+          float v[8];
+          k.get_mirrored(r0, v);
+          epilogue8(e, alpha, beta, c_exp, n0 + 16 * j + 8 * (lane & 1), m0 + r0 + (lane >> 1), z, v);
+        }
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
   }
   if (e.sums != nullptr) {
     // Lanes with the same rows add up in a fixed order; one partial row per wave column.
+    constexpr int LPC = Parked<S>::LPC;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -221,7 +322,7 @@ __device__ inline void finish_tile(const Gemm16Args& p, unsigned char* lds, int 
       float* out = e.sums + (long)(tile_n * S::WGN + wave / S::WGM) * e.rows;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (m0 + wm0 + er + i < e.rows) out[m0 + wm0 + er + i] = sums[i];
+        if (m0 + k.row + i < e.rows) out[m0 + k.row + i] = sums[i];
     }
   }
 }
@@ -328,7 +429,7 @@ struct Dma16 {
     return u4_t{(unsigned)at, (unsigned)(at >> 32) & 0xffffu, 0xffffffffu, 0x00020000u};
   }
 };
-__device__ inline unsigned lds_address(const unsigned char* p) {
+[[maybe_unused]] __device__ inline unsigned lds_address(const unsigned char* p) {
   return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p;
 }
 
@@ -562,7 +663,6 @@ rtat_status_t launch_gemm16(rtat_native_handle* h, const Gemm16& g) {
   p.ldb = g.ldb;
   p.b_stride = g.b_stride;
   p.ep = g.ep;
-  settle_vec(p.ep);
   return g.type == RTAT_TYPE_BF16 ? launch_type<__bf16>(h, g, p) : launch_type<_Float16>(h, g, p);
 }
 

@@ -15,7 +15,7 @@ namespace {
 constexpr int ROWS = 128, COLS = 16;  // rows and columns a workgroup holds at a time
 
 struct ActArgs {
-  int type, act, m, n, per_chunk, vec;
+  int type, act, m, n, per_chunk;
   const uint16_t* dD;
   long lddd;
   const uint16_t* Z;
@@ -36,15 +36,14 @@ __global__ __launch_bounds__(256) void act_backward_kernel(ActArgs p) {
   for (int i = 0; i < 8; ++i) sums[i] = 0.0f;
   const bool slope = p.act != RTAT_ACT_NONE;
   if (row < p.m) {
-    if (p.vec && row + 8 <= p.m) {
+    if (row + 8 <= p.m) {
 #pragma unroll 4
       for (int col = first + lc; col < last; col += COLS) {
         float v[8], z[8];
         load8(p.type, p.dD, row + (long)col * p.lddd, v);
         if (slope) {
           load8(p.type, p.Z, row + (long)col * p.ldz, z);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] *= act_slope(p.act, z[i]);
+          act_slopes(p.act, z, v);
           if (p.dZ != nullptr) store8(p.type, p.dZ, row + (long)col * p.lddz, v);
         }
 #pragma unroll
@@ -98,8 +97,6 @@ rtat_status_t launch_act_backward(rtat_native_handle* h, int type, int act, int 
   p.ldz = ldz;
   p.dZ = static_cast<uint16_t*>(dZ);
   p.lddz = lddz;
-  p.vec = vec_ok(dD, lddd, 0, type) && vec_ok(act != RTAT_ACT_NONE ? Z : nullptr, ldz, 0, type) &&
-          vec_ok(dZ, lddz, 0, type);
   const long strips = (m + ROWS - 1) / ROWS;
   // Enough chunks for eight workgroups per CU, none shorter than four passes; never more rows of
   // partial sums than dbias_workspace_bytes counts (one per 32 columns).

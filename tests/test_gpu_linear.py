@@ -92,6 +92,39 @@ def test_forward_ops_and_sizes(handle, ta, tb, size):
         assert D.padding_kept() and Z.padding_kept()
 
 
+@pytest.mark.parametrize("ta", [N, T])
+@pytest.mark.parametrize("tb", [N, T])
+@pytest.mark.parametrize("size", [(3001, 3003, 129), (3000, 3080, 200), (2817, 4096, 64), (4096, 2816, 72), (3333, 2900, 1),
+                                  (2560, 3584, 640)])
+def test_forward_many_tiles(handle, ta, tb, size):
+    """Enough tiles for the largest tile shape, 16-byte aligned columns, ragged edges and k."""
+    m, n, k = size
+    for which in ("bf16", "f16"):
+        dt, ty = _types()[which]
+        gen = _gen(m + n)
+        A = Mat(*((k, m) if ta == T else (m, k)), dt, 0, 0, gen, k ** -0.5)
+        B = Mat(*((n, k) if tb == T else (k, n)), dt, 0, 0, gen)
+        A, B = (Mat(x.m.shape[0], x.m.shape[1], dt, -x.m.shape[0] % 8, 0, gen) for x in (A, B))
+        C, D, Z = Mat(m, n, dt, 1, 0, gen), Mat(m, n, dt, 5), Mat(m, n, dt, -m % 8)
+        handle.gemm_ep(ty, ta, tb, m, n, k, 0.5, A.ptr, A.ld, B.ptr, B.ld, D.ptr, D.ld, act=ref.SILU, aux=Z.ptr, ldaux=Z.ld,
+                       beta=1.0, C=C.ptr, ldc=C.ld)
+        (y, yb), (z, zb) = ref.forward(0.5, _op(A.m, ta), _op(B.m, tb), k, None, ref.SILU, 1.0, C.m, dt, dt)
+        assert _within(D.m, y, yb) and _within(Z.m, z, zb)
+        assert D.padding_kept() and Z.padding_kept()
+        # the gradient's form of the same product, sums of many columns
+        db = torch_empty(m)
+        handle.gemm_dact(ty, ta, tb, m, n, k, 0.5, A.ptr, A.ld, B.ptr, B.ld, ref.GELU, C.ptr, C.ld, D.ptr, D.ld, dbias=db)
+        g, e = ref.product(0.5, _op(A.m, ta), _op(B.m, tb), k)
+        want, e = g * ref.slope(C.m.double(), ref.GELU), 1.13 * e + 2 * (ref.SLOPE_ERR + ref.U) * g.abs()
+        assert _within(D.m, want, ref.rounded(want, e, dt)) and D.padding_kept()
+        assert _within(db, want.sum(1), e.sum(1) + (n + 2) * ref.U * want.abs().sum(1))
+
+
+def torch_empty(m):
+    import torch
+    return torch.full((m,), float("nan"), device="cuda")
+
+
 @pytest.mark.parametrize("act", range(5))
 @pytest.mark.parametrize("which", ["bf16", "f16"])
 def test_forward_activations(handle, act, which):

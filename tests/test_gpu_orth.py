@@ -58,6 +58,14 @@ def test_shapes(handle, which, kind, m, n):
     _check(src, O, coeffs)
 
 
+@pytest.mark.parametrize("m,n", [(4100, 4200), (4250, 4099)])
+def test_large(handle, m, n):
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    src, O = _run(handle, "bf16", _update(gen, 1, n, m, "strong"), [QUINTIC] * 5)
+    _check(src, O, [QUINTIC] * 5)
+
+
 @pytest.mark.parametrize("steps", [1, 2, 3, 6])
 def test_steps_and_other_coefficients(handle, steps):
     import torch
