@@ -13,9 +13,9 @@
 //     each read over the LDS banks.  Measured clocks per wave instruction, 16 waves of a CU
 //     reading: 16 bytes per lane 3.8 with it, 10.3 without; transposing 2.9 with it, 11.0
 //     without (row strides of 128 and 512 bytes).
-//   * The accumulators pass through LDS one block column at a time, which turns them into eight
-//     neighbouring rows per lane: bias, residual, saved activations and results move in 16-byte
-//     accesses, and the epilogue is one rolled loop whatever it has to do.
+//   * The epilogue turns accumulators into eight neighbouring rows per lane, so that bias,
+//     residual, saved activations and results move in 16-byte accesses: by exchanges between
+//     lanes in a tile that lies inside C, through LDS in one that hangs over its edge.
 #include <type_traits>
 
 #include "gemm16.h"
@@ -37,7 +37,7 @@ struct Gemm16Args {
 
 constexpr int BK16 = 64;
 
-template <int BM_, int BN_, int WGM_, int WGN_, int OCC_>
+template <int BM_, int BN_, int WGM_, int WGN_, int OCC_, bool RING_ = false>
 struct Shape16 {
   static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, OCC = OCC_;
   static constexpr int NW = WGM * WGN, NT = 64 * NW;
@@ -45,7 +45,8 @@ struct Shape16 {
   static constexpr int TM = WTM / 16, TN = WTN / 16;    // MFMA blocks per wave tile
   static constexpr int STAGE = (BM + BN) * BK16 * 2;    // bytes
   static constexpr int PARK = WTM + 4;                  // floats per parked column
-  static constexpr int LDS = 2 * STAGE > NW * 16 * PARK * 4 ? 2 * STAGE : NW * 16 * PARK * 4;
+  static constexpr int LDS = RING_ ? 5 * BM * BK16 * 2 : 2 * STAGE;  // five panels, or two stages
+  static_assert(LDS >= NW * 16 * PARK * 4, "room to park a block column per wave");
 };
 
 // A panel of ROWS x 64 elements in LDS, in bytes.
@@ -147,8 +148,8 @@ struct Mover16 {
   }
 };
 
-// The epilogue of a tile, a block column (16 columns of C) at a time: the wave parks it in its own
-// part of LDS, column by column, and takes it back as eight neighbouring rows per lane.
+// A block column (16 columns of C) of a wave tile on its way through the wave's own part of LDS:
+// parked column by column, taken back as eight neighbouring rows per lane or as the mirror image.
 template <class S>
 struct Parked {
   static constexpr int LPC = S::WTM / 8;   // lanes per column
@@ -195,14 +196,43 @@ struct Parked {
   }
 };
 
+// Two accumulators of neighbouring blocks, 16 rows apart, exchanged between neighbouring groups of
+// 16 lanes, so that x and y become the first and second four of eight neighbouring rows of the
+// lane's column: rows 16 (q % 2) + 8 (q / 2) .. + 7 of the pair's 32, q = lane / 16.
+__device__ inline void pair_up(float& x, float& y) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x),
+                                                  __builtin_bit_cast(unsigned, y), false, false);
+  const unsigned lo = r[0], hi = r[1];
+  x = __builtin_bit_cast(float, lo);
+  y = __builtin_bit_cast(float, hi);
+}
+
+// Block column j, J <= j < TN, of a wave tile as TM / 2 times eight neighbouring rows.
+template <class S, int J = 0>
+__device__ __forceinline__ void take(int j, const f4_t (&acc)[S::TM][S::TN],
+                                     float (&v)[S::TM / 2][8]) {
+  if (j == J) {  // the accumulators must be named by constants
+#pragma unroll
+    for (int q = 0; q < S::TM / 2; ++q)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        v[q][r] = acc[2 * q][J][r];
+        v[q][4 + r] = acc[2 * q + 1][J][r];
+      }
+  } else if constexpr (J + 1 < S::TN) {
+    take<S, J + 1>(j, acc, v);
+  }
+}
+
 // A tile that lies wholly inside C: nothing to check, and what a block column needs from memory
-// (the residual, or the argument of the activation) is asked for one block column ahead.
+// (the residual, or the argument of the activation) is asked for one block column ahead.  The
+// accumulators stay in registers: a store instruction covers 64 neighbouring bytes of 16 columns.
 template <class S, bool SLOPE>
-__device__ __forceinline__ void finish_inside(const Epilogue& e, const Parked<S>& k, float alpha, float beta,
-                                     int c_exp, int m0, int n0, long z,
-                                     const f4_t (&acc)[S::TM][S::TN], float (&sums)[8]) {
-  constexpr int PASSES = Parked<S>::PASSES;
-  const int row = m0 + k.row, col = n0 + k.col;
+__device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float alpha, float beta,
+                                              int c_exp, int m0, int n0, long z, float* sums_out,
+                                              const f4_t (&acc)[S::TM][S::TN]) {
+  constexpr int NP = S::TM / 2;
+  const int row = m0 + 16 * ((lane >> 4) & 1) + 8 * (lane >> 5), col = n0 + (lane & 15);
   const void* in = SLOPE ? (e.act != RTAT_ACT_NONE ? e.aux : nullptr) : e.C;
   const int in_type = SLOPE ? e.aux_type : e.c_type;
   const long ldin = SLOPE ? e.ldaux : e.ldc;
@@ -210,42 +240,45 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, const Parked<S>
   const long d0 = z * e.d_stride + row + col * e.ldd;
   const long aux0 = z * e.aux_stride + row + col * e.ldaux;
   const long copy0 = z * e.copy_stride + row + col * e.ldcopy;
-  float bias[8];
+  float each[NP][8];  // the rows' bias, or their sums
 #pragma unroll
-  for (int i = 0; i < 8; ++i) bias[i] = 0.0f;
-  if (!SLOPE && e.bias != nullptr) load8(e.bias_type, e.bias, row, bias);
-  Raw8 next[PASSES];
+  for (int q = 0; q < NP; ++q) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) each[q][i] = 0.0f;
+    if (!SLOPE && e.bias != nullptr) load8(e.bias_type, e.bias, row + 32 * q, each[q]);
+  }
+  Raw8 next[NP];
   auto ask = [&](int j) {
     if (in != nullptr) {
 #pragma unroll
-      for (int q = 0; q < PASSES; ++q)
-        next[q] = fetch8(in_type, in, in0 + (16 * j + q * Parked<S>::CPP) * ldin);
+      for (int q = 0; q < NP; ++q) next[q] = fetch8(in_type, in, in0 + 32 * q + 16 * j * ldin);
     }
   };
   ask(0);
 #pragma unroll 1
   for (int j = 0; j < S::TN; ++j) {
-    k.put(j, acc);
-    Raw8 now[PASSES];
+    Raw8 now[NP];
 #pragma unroll
-    for (int q = 0; q < PASSES; ++q) now[q] = next[q];
+    for (int q = 0; q < NP; ++q) now[q] = next[q];
     if (j + 1 < S::TN) ask(j + 1);
-    float v[PASSES][8];
+    float v[NP][8];
+    take<S>(j, acc, v);
 #pragma unroll
-    for (int q = 0; q < PASSES; ++q) k.get(q, v[q]);
+    for (int q = 0; q < NP; ++q) {
 #pragma unroll
-    for (int q = 0; q < PASSES; ++q) {
-      const long c = 16 * j + q * Parked<S>::CPP;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[q][i] = __builtin_fmaf(v[q][i], alpha, bias[i]);
+      for (int r = 0; r < 4; ++r) pair_up(v[q][r], v[q][4 + r]);
       float w[8];
       if (in != nullptr) unpack8(in_type, now[q], w);
       if constexpr (SLOPE) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[q][i] *= alpha;
         if (in != nullptr) act_slopes(e.act, w, v[q]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sums[i] += v[q][i];
+        for (int i = 0; i < 8; ++i) each[q][i] += v[q][i];
       } else {
-        if (e.aux != nullptr) store8(e.aux_type, e.aux, aux0 + c * e.ldaux, v[q]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[q][i] = __builtin_fmaf(v[q][i], alpha, each[q][i]);
+        if (e.aux != nullptr) store8(e.aux_type, e.aux, aux0 + 32 * q + 16 * j * e.ldaux, v[q]);
         act_values(e.act, v[q]);
         if (in != nullptr) {
           if (c_exp != 0) {
@@ -256,8 +289,21 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, const Parked<S>
           for (int i = 0; i < 8; ++i) v[q][i] = __builtin_fmaf(beta, w[i], v[q][i]);
         }
       }
-      store8(e.d_type, e.D, d0 + c * e.ldd, v[q]);
-      if (!SLOPE && e.copy != nullptr) store8(RTAT_TYPE_F16, e.copy, copy0 + c * e.ldcopy, v[q]);
+      store8(e.d_type, e.D, d0 + 32 * q + 16 * j * e.ldd, v[q]);
+      if (!SLOPE && e.copy != nullptr)
+        store8(RTAT_TYPE_F16, e.copy, copy0 + 32 * q + 16 * j * e.ldcopy, v[q]);
+    }
+  }
+  if (SLOPE && sums_out != nullptr) {
+    // The sixteen columns add up in a fixed order.
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) each[q][i] += __shfl_xor(each[q][i], d);
+      if ((lane & 15) == 0)
+        store8(RTAT_TYPE_F32, sums_out, row + 32 * q, each[q]);
     }
   }
 }
@@ -279,20 +325,25 @@ __device__ __forceinline__ void finish_tile(const Gemm16Args& p, unsigned char* 
       c_exp = (int)e.scale[2 * z + 1];
     }
   }
+  // One row of partial sums per wave column.
+  float* sums_out =
+      e.sums != nullptr ? e.sums + (long)(tile_n * S::WGN + wave / S::WGM) * e.rows : nullptr;
+  const bool mirror = p.tri != 0 && tile_m != tile_n;
+  const bool inside = m0 + S::WTM <= e.rows && n0 + S::WTN <= e.cols &&
+                      (e.C == nullptr || (m0 + S::WTM <= e.c_rows && n0 + S::WTN <= e.c_cols));
+  if (inside) {
+    if (e.slope) finish_inside<S, true>(e, lane, alpha, beta, c_exp, m0, n0, z, sums_out, acc);
+    else finish_inside<S, false>(e, lane, alpha, beta, c_exp, m0, n0, z, sums_out, acc);
+    if (!mirror) return;
+  }
   const Parked<S> k(lds, wave, lane);
   float sums[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) sums[i] = 0.0f;
-  const bool mirror = p.tri != 0 && tile_m != tile_n;
-  const bool inside = m0 + S::WTM <= e.rows && n0 + S::WTN <= e.cols &&
-                      (e.C == nullptr || (m0 + S::WTM <= e.c_rows && n0 + S::WTN <= e.c_cols));
-  if (inside && !mirror) {
-    if (e.slope) finish_inside<S, true>(e, k, alpha, beta, c_exp, m0, n0, z, acc, sums);
-    else finish_inside<S, false>(e, k, alpha, beta, c_exp, m0, n0, z, acc, sums);
-  } else {
 #pragma unroll 1
-    for (int j = 0; j < S::TN; ++j) {
-      k.put(j, acc);
+  for (int j = 0; j < S::TN; ++j) {
+    k.put(j, acc);
+    if (!inside) {
 #pragma unroll 1
       for (int q = 0; q < Parked<S>::PASSES; ++q) {
         float v[8];
@@ -301,28 +352,27 @@ __device__ __forceinline__ void finish_tile(const Gemm16Args& p, unsigned char* 
 #pragma unroll
         for (int i = 0; i < 8; ++i) sums[i] += v[i];
       }
-      if (mirror) {
+    }
+    if (mirror) {
 #pragma unroll 1
-        for (int r0 = 0; r0 < S::WTM; r0 += 32) {
-          float v[8];
-          k.get_mirrored(r0, v);
-          epilogue8(e, alpha, beta, c_exp, n0 + 16 * j + 8 * (lane & 1), m0 + r0 + (lane >> 1), z, v);
-        }
+      for (int r0 = 0; r0 < S::WTM; r0 += 32) {
+        float v[8];
+        k.get_mirrored(r0, v);
+        epilogue8(e, alpha, beta, c_exp, n0 + 16 * j + 8 * (lane & 1), m0 + r0 + (lane >> 1), z, v);
       }
     }
   }
-  if (e.sums != nullptr) {
-    // Lanes with the same rows add up in a fixed order; one partial row per wave column.
+  if (sums_out != nullptr) {
+    // Lanes with the same rows add up in a fixed order.
     constexpr int LPC = Parked<S>::LPC;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int d = LPC; d < 64; d *= 2) sums[i] += __shfl_xor(sums[i], d);
     if (lane < LPC) {
-      float* out = e.sums + (long)(tile_n * S::WGN + wave / S::WGM) * e.rows;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (m0 + k.row + i < e.rows) out[m0 + k.row + i] = sums[i];
+        if (m0 + k.row + i < e.rows) sums_out[m0 + k.row + i] = sums[i];
     }
   }
 }
@@ -416,7 +466,7 @@ struct Dma16 {
   // Instruction i of a panel (`where`: panel_at).  Written in assembly because behind the builtin
   // the compiler waits for every load in flight before each transposing LDS read (the s_nop is the
   // wait state between M0 and a load to LDS); it has no
-  // result register, and wait_all_and_meet is its wait; nothing else here reads M0.
+  // result register, and wait_and_meet is its wait; nothing else here reads M0.
   __device__ inline void issue(int i, u4_t where, unsigned panel, int wave) const {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
@@ -433,11 +483,12 @@ struct Dma16 {
   return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p;
 }
 
-// Everything this wave asked for has arrived and everything it read is in registers; then the
+// All but the wave's last N loads have arrived and everything it read is in registers; then the
 // same of all waves.
-[[maybe_unused]] __device__ inline void wait_all_and_meet() {
+template <int N>
+[[maybe_unused]] __device__ inline void wait_and_meet() {
   __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
   __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -445,10 +496,14 @@ struct Dma16 {
 //   * A wave holds 128 x 128 of C in 256 accumulator registers, which needs the fewest LDS bytes
 //     per MFMA (32 reads of 1 KiB for 128 MFMAs of 16 clocks; eight waves of 128 x 64 would ask LDS
 //     for 48 in the time it delivers 48).
-//   * Panel kt + 2 is on its way into the stage that panel kt just left while panel kt + 1 is
-//     computed: loads go straight to LDS, so they cost no registers.  One barrier per panel, half
-//     way through it: by then the second half's operands are in registers, so the stage is free,
-//     and the next panel, asked for one panel ago, has arrived.
+//   * Panels go straight to LDS, so loads in flight cost no registers.  LDS holds a ring of five
+//     32 KiB slots, A and B panels alternating: while panel kt is computed, panel kt + 1 is there
+//     or on its way, A of panel kt + 2 is asked for in the first half of kt (the fifth slot) and
+//     B in the second half (a slot that kt just left), eight loads in each half.  Loads are so
+//     evenly spread that a wave, alone on its SIMD, hardly waits to issue them (all sixteen in one
+//     half, into two 64 KiB stages: 8192^3 830 us; bunched at its start 865).
+//   * One barrier per panel, half way through it: by then the second half's operands are in
+//     registers, so both slots are free, and of the loads only the last eight may be missing.
 //   * Within a half the LDS reads of the next half and the panel loads are spread behind the
 //     MFMAs one by one.
 template <class T, class S, bool KA, bool KB>
@@ -484,24 +539,26 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
   const int panels = (p.k + BK16 - 1) / BK16;
   const bool ragged = p.k % BK16 != 0 || (!KA && m0 + S::BM > p.m) || (!KB && n0 + S::BN > p.n);
   const int whole = panels - (ragged ? 1 : 0);
+  // Item 2 kt is A of panel kt, item 2 kt + 1 its B; item x lies in slot x % 5.
+  static_assert(S::BM == S::BN && S::LDS >= 5 * PA::BYTES, "slots of one size");
+  auto slot = [&](int item) { return lds + (item % 5) * PA::BYTES; };
   auto issue_all = [&](int kt) {
-    unsigned char* stage = lds + (kt & 1) * S::STAGE;
     if (kt < whole) {
       const u4_t pa = da.panel_at(At, p.lda, kt), pb = db.panel_at(Bt, p.ldb, kt);
-      const unsigned to = lds_address(stage);
+      const unsigned to_a = lds_address(slot(2 * kt)), to_b = lds_address(slot(2 * kt + 1));
 #pragma unroll
-      for (int i = 0; i < da.NI; ++i) da.issue(i, pa, to, wave);
+      for (int i = 0; i < da.NI; ++i) da.issue(i, pa, to_a, wave);
 #pragma unroll
-      for (int i = 0; i < db.NI; ++i) db.issue(i, pb, to + PA::BYTES, wave);
+      for (int i = 0; i < db.NI; ++i) db.issue(i, pb, to_b, wave);
     } else {
       {
         Mover16<KA, S::BM, S::NT> ma;
         ma.load(A, p.lda, m0, p.m, kt * BK16, p.k, t);
-        ma.store(stage, t);
+        ma.store(slot(2 * kt), t);
       }
       Mover16<KB, S::BN, S::NT> mb;
       mb.load(B, p.ldb, n0, p.n, kt * BK16, p.k, t);
-      mb.store(stage + PA::BYTES, t);
+      mb.store(slot(2 * kt + 1), t);
     }
   };
 
@@ -509,15 +566,14 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
   const Frags16<KB, S::BN> rb(wn0, lane);
   s8_t fa[2][TM], fb[2][TN];
   // Operand x of a K-step, in the order the MFMAs want them: the first row of A, B, the other rows.
-  auto read = [&](int stage, int step, int x) {
-    const unsigned char* at = lds + stage * S::STAGE;
-    if (x == 0 || x > TN) fa[step][x == 0 ? 0 : x - TN] = ra.read(at, x == 0 ? 0 : x - TN, step);
-    else fb[step][x - 1] = rb.read(at + PA::BYTES, x - 1, step);
+  auto read = [&](const unsigned char* pa, const unsigned char* pb, int step, int x) {
+    if (x == 0 || x > TN) fa[step][x == 0 ? 0 : x - TN] = ra.read(pa, x == 0 ? 0 : x - TN, step);
+    else fb[step][x - 1] = rb.read(pb, x - 1, step);
   };
-  // The MFMAs of one K-step with `side(x)`, x = 0 .. TM + TN - 1, spread behind the first three
-  // quarters of them.
-  auto multiply = [&](int step, auto side) {
-    constexpr int GAP = 3 * TM * TN / (4 * (TM + TN));
+  // The MFMAs of one K-step, with read(x), x = 0 .. TM + TN - 1, spread behind the first three
+  // quarters of them and load(i), i = 0 .. 7, behind all.
+  auto multiply = [&](int step, auto read_x, auto load_i) {
+    constexpr int NMFMA = TM * TN, GAP = 3 * NMFMA / (4 * (TM + TN)), LOAD_GAP = NMFMA / 8;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -525,40 +581,41 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
         const int x = i * TN + j;
         Half<T>::mfma_into(acc[i][j], fa[step][i], fb[step][j]);
         if (x % GAP == 0 && x / GAP < TM + TN) {
-          side(x / GAP);
+          read_x(x / GAP);
           __builtin_amdgcn_sched_barrier(0);
         }
+        if (x % LOAD_GAP == LOAD_GAP / 2) load_i(x / LOAD_GAP);
       }
   };
-  static_assert(TM + TN == decltype(da)::NI + decltype(db)::NI, "a load goes with every LDS read");
+  static_assert(decltype(da)::NI == 8 && decltype(db)::NI == 8, "eight loads a panel");
+  auto no_load = [](int) {};
 
   if (panels > 0) {
     issue_all(0);
-    wait_all_and_meet();
     if (panels > 1) issue_all(1);
+    if (whole > 1) wait_and_meet<16>();
+    else wait_and_meet<0>();
 #pragma unroll
-    for (int x = 0; x < TM + TN; ++x) read(0, 0, x);
+    for (int x = 0; x < TM + TN; ++x) read(slot(0), slot(1), 0, x);
   }
   int kt = 0;
   for (; kt < whole - 2; ++kt) {
-    const int cur = kt & 1, nxt = cur ^ 1;
-    multiply(0, [&](int x) { read(cur, 1, x); });
-    wait_all_and_meet();
-    const unsigned to = lds_address(lds + cur * S::STAGE);
+    const unsigned char *a0 = slot(2 * kt), *b0 = slot(2 * kt + 1);
+    const unsigned char *a1 = slot(2 * kt + 2), *b1 = slot(2 * kt + 3);
     const u4_t pa = da.panel_at(At, p.lda, kt + 2), pb = db.panel_at(Bt, p.ldb, kt + 2);
-    multiply(1, [&](int x) {
-      if (x < da.NI) da.issue(x, pa, to, wave);
-      else db.issue(x - da.NI, pb, to + PA::BYTES, wave);
-      read(nxt, 0, x);
-    });
+    const unsigned to_a = lds_address(slot(2 * kt + 4)), to_b = lds_address(a0);
+    multiply(0, [&](int x) { read(a0, b0, 1, x); }, [&](int i) { da.issue(i, pa, to_a, wave); });
+    wait_and_meet<8>();
+    multiply(1, [&](int x) { read(a1, b1, 0, x); }, [&](int i) { db.issue(i, pb, to_b, wave); });
   }
 #pragma unroll 1
   for (; kt < panels; ++kt) {
-    const int cur = kt & 1, nxt = cur ^ 1;
-    multiply(0, [&](int x) { read(cur, 1, x); });
-    wait_all_and_meet();
+    const unsigned char *a0 = slot(2 * kt), *b0 = slot(2 * kt + 1);
+    const unsigned char *a1 = slot(2 * kt + 2), *b1 = slot(2 * kt + 3);
+    multiply(0, [&](int x) { read(a0, b0, 1, x); }, no_load);
+    wait_and_meet<0>();
     if (kt + 2 < panels) issue_all(kt + 2);
-    multiply(1, [&](int x) { read(nxt, 0, x); });  // of the last panel: not used
+    multiply(1, [&](int x) { read(a1, b1, 0, x); }, no_load);  // of the last panel: not used
   }
   mfma_settle();
   __syncthreads();
@@ -566,7 +623,7 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
 #endif
 }
 
-typedef Shape16<256, 256, 2, 2, 1> S256x256;  // loads straight to LDS
+typedef Shape16<256, 256, 2, 2, 1, true> S256x256;  // loads straight to LDS
 typedef Shape16<128, 128, 2, 2, 2> S128x128;
 typedef Shape16<64, 64, 2, 2, 4> S64x64;
 
