@@ -169,34 +169,18 @@ __device__ inline u4_t pack8(int type, const float (&v)[8]) {
   for (int e = 0; e < 8; ++e) h[e] = (_Float16)v[e];
   return __builtin_bit_cast(u4_t, h);
 }
-// The bits of eight elements from element i on; `hi` only for F32.
-struct Raw8 {
-  u4_t lo, hi;
-};
-__device__ inline Raw8 fetch8(int type, const void* p, long i) {
-  Raw8 r = {};
+__device__ inline void load8(int type, const void* p, long i, float (&v)[8]) {
   if (type == RTAT_TYPE_F32) {
-    r.lo = load16(p, 4 * i);
-    r.hi = load16(p, 4 * i + 16);
-  } else {
-    r.lo = load16(p, 2 * i);
-  }
-  return r;
-}
-__device__ inline void unpack8(int type, const Raw8& r, float (&v)[8]) {
-  if (type == RTAT_TYPE_F32) {
-    const f4_t a = __builtin_bit_cast(f4_t, r.lo), b = __builtin_bit_cast(f4_t, r.hi);
+    const f4_t a = __builtin_bit_cast(f4_t, load16(p, 4 * i));
+    const f4_t b = __builtin_bit_cast(f4_t, load16(p, 4 * i + 16));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[e] = a[e];
       v[4 + e] = b[e];
     }
   } else {
-    unpack8(type, r.lo, v);
+    unpack8(type, load16(p, 2 * i), v);
   }
-}
-__device__ inline void load8(int type, const void* p, long i, float (&v)[8]) {
-  unpack8(type, fetch8(type, p, i), v);
 }
 __device__ inline void store8(int type, void* p, long i, const float (&v)[8]) {
   if (type == RTAT_TYPE_F32) {
@@ -207,11 +191,40 @@ __device__ inline void store8(int type, void* p, long i, const float (&v)[8]) {
   }
 }
 
-// Eight elements through an activation; the choice is made once for all of them.
-__device__ inline void act_values(int act, float (&v)[8]) {
-#define RTAT_EACH(A)                                                    \
-  case A:                                                               \
-    _Pragma("unroll") for (int i = 0; i < 8; ++i) v[i] = act_value(A, v[i]); \
+// N times eight 16-bit elements; one choice of type for all.
+template <int N>
+__device__ inline void unpack_all(int type, const u4_t (&r)[N], float (&v)[N][8]) {
+  if (type == RTAT_TYPE_BF16) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) unpack8(RTAT_TYPE_BF16, r[q], v[q]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < N; ++q) unpack8(RTAT_TYPE_F16, r[q], v[q]);
+  }
+}
+// N times eight elements, 32 apart, from element i on.
+template <int N>
+__device__ inline void store_all(int type, void* p, long i, const float (&v)[N][8]) {
+  if (type == RTAT_TYPE_BF16) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) store8(RTAT_TYPE_BF16, p, i + 32 * q, v[q]);
+  } else if (type == RTAT_TYPE_F16) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) store8(RTAT_TYPE_F16, p, i + 32 * q, v[q]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < N; ++q) store8(RTAT_TYPE_F32, p, i + 32 * q, v[q]);
+  }
+}
+
+// N times eight elements through an activation; the choice is made once for all of them.
+template <int N>
+__device__ inline void act_values(int act, float (&v)[N][8]) {
+#define RTAT_EACH(A)                                     \
+  case A:                                                \
+    _Pragma("unroll") for (int q = 0; q < N; ++q)        \
+      _Pragma("unroll") for (int i = 0; i < 8; ++i)      \
+        v[q][i] = act_value(A, v[q][i]);                 \
     break;
   switch (act) {
     RTAT_EACH(RTAT_ACT_RELU)
@@ -223,10 +236,13 @@ __device__ inline void act_values(int act, float (&v)[8]) {
 #undef RTAT_EACH
 }
 // v *= act'(z)
-__device__ inline void act_slopes(int act, const float (&z)[8], float (&v)[8]) {
-#define RTAT_EACH(A)                                                          \
-  case A:                                                                     \
-    _Pragma("unroll") for (int i = 0; i < 8; ++i) v[i] *= act_slope(A, z[i]); \
+template <int N>
+__device__ inline void act_slopes(int act, const float (&z)[N][8], float (&v)[N][8]) {
+#define RTAT_EACH(A)                                     \
+  case A:                                                \
+    _Pragma("unroll") for (int q = 0; q < N; ++q)        \
+      _Pragma("unroll") for (int i = 0; i < 8; ++i)      \
+        v[q][i] *= act_slope(A, z[q][i]);                \
     break;
   switch (act) {
     RTAT_EACH(RTAT_ACT_RELU)
@@ -264,6 +280,7 @@ struct Epilogue {
   float* sums;  // gradient: one row of `rows` partial sums per wave column of the launch
   const float* scale;
   int r_power, scale_c;
+  int plain;  // nothing but alpha, and D has the operands' type (set by launch_gemm16)
 };
 
 // Rows row .. row + 7 of column col, batch matrix z: v holds the accumulators and, for a
@@ -285,7 +302,7 @@ __device__ inline void epilogue8(const Epilogue& e, float alpha, float beta, int
     if (e.slope) {
       if (e.act != RTAT_ACT_NONE) {
         load8(e.aux_type, e.aux, aux_at, w);
-        act_slopes(e.act, w, v);
+        act_slopes<1>(e.act, reinterpret_cast<const float(&)[1][8]>(w), reinterpret_cast<float(&)[1][8]>(v));
       }
     } else {
       float c[8];
@@ -297,7 +314,7 @@ __device__ inline void epilogue8(const Epilogue& e, float alpha, float beta, int
         for (int i = 0; i < 8; ++i) v[i] += w[i];
       }
       if (e.aux != nullptr) store8(e.aux_type, e.aux, aux_at, v);
-      act_values(e.act, v);
+      act_values<1>(e.act, reinterpret_cast<float(&)[1][8]>(v));
       if (with_c) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(beta, __builtin_ldexpf(c[i], c_exp), v[i]);

@@ -207,26 +207,32 @@ __device__ inline void pair_up(float& x, float& y) {
   y = __builtin_bit_cast(float, hi);
 }
 
-// Block column j, J <= j < TN, of a wave tile as TM / 2 times eight neighbouring rows.
-template <class S, int J = 0>
+// Block column J of a wave tile as TM / 2 times eight neighbouring rows, 32 apart.
+template <class S, int J>
+__device__ __forceinline__ void take_one(const f4_t (&acc)[S::TM][S::TN], float (&v)[S::TM / 2][8]) {
+#pragma unroll
+  for (int q = 0; q < S::TM / 2; ++q)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      v[q][r] = acc[2 * q][J][r];
+      v[q][4 + r] = acc[2 * q + 1][J][r];
+    }
+  asm volatile("; block column %0" : : "n"(J));  // keeps the compiler from merging the copies of this
+}
+// Block column j, LO <= j < HI: the accumulators must be named by constants.
+template <class S, int LO = 0, int HI = S::TN>
 __device__ __forceinline__ void take(int j, const f4_t (&acc)[S::TM][S::TN],
                                      float (&v)[S::TM / 2][8]) {
-  if (j == J) {  // the accumulators must be named by constants
-#pragma unroll
-    for (int q = 0; q < S::TM / 2; ++q)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        v[q][r] = acc[2 * q][J][r];
-        v[q][4 + r] = acc[2 * q + 1][J][r];
-      }
-  } else if constexpr (J + 1 < S::TN) {
-    take<S, J + 1>(j, acc, v);
-  }
+  if constexpr (HI - LO == 1) take_one<S, LO>(acc, v);
+  else if (j < (LO + HI) / 2) take<S, LO, (LO + HI) / 2>(j, acc, v);
+  else take<S, (LO + HI) / 2, HI>(j, acc, v);
 }
 
 // A tile that lies wholly inside C: nothing to check, and what a block column needs from memory
 // (the residual, or the argument of the activation) is asked for one block column ahead.  The
 // accumulators stay in registers: a store instruction covers 64 neighbouring bytes of 16 columns.
+// A wave of the largest tile is alone on its SIMD and waits out every taken branch, so choices
+// are made once per block column.
 template <class S, bool SLOPE>
 __device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float alpha, float beta,
                                               int c_exp, int m0, int n0, long z, float* sums_out,
@@ -236,10 +242,10 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float
   const void* in = SLOPE ? (e.act != RTAT_ACT_NONE ? e.aux : nullptr) : e.C;
   const int in_type = SLOPE ? e.aux_type : e.c_type;
   const long ldin = SLOPE ? e.ldaux : e.ldc;
-  const long in0 = z * (SLOPE ? e.aux_stride : e.c_stride) + row + col * ldin;
-  const long d0 = z * e.d_stride + row + col * e.ldd;
-  const long aux0 = z * e.aux_stride + row + col * e.ldaux;
-  const long copy0 = z * e.copy_stride + row + col * e.ldcopy;
+  long in_at = z * (SLOPE ? e.aux_stride : e.c_stride) + row + col * ldin;
+  long d_at = z * e.d_stride + row + col * e.ldd;
+  long aux_at = z * e.aux_stride + row + col * e.ldaux;
+  long copy_at = z * e.copy_stride + row + col * e.ldcopy;
   float each[NP][8];  // the rows' bias, or their sums
 #pragma unroll
   for (int q = 0; q < NP; ++q) {
@@ -247,51 +253,70 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float
     for (int i = 0; i < 8; ++i) each[q][i] = 0.0f;
     if (!SLOPE && e.bias != nullptr) load8(e.bias_type, e.bias, row + 32 * q, each[q]);
   }
-  Raw8 next[NP];
-  auto ask = [&](int j) {
-    if (in != nullptr) {
+  // Sixteen-bit values are asked for ahead; 32-bit ones would take twice the registers.
+  const bool ahead = in != nullptr && in_type != RTAT_TYPE_F32;
+  u4_t next[NP];
 #pragma unroll
-      for (int q = 0; q < NP; ++q) next[q] = fetch8(in_type, in, in0 + 32 * q + 16 * j * ldin);
-    }
-  };
-  ask(0);
+  for (int q = 0; q < NP; ++q) next[q] = ahead ? load16(in, 2 * (in_at + 32 * q)) : u4_t{};
 #pragma unroll 1
   for (int j = 0; j < S::TN; ++j) {
-    Raw8 now[NP];
+    u4_t now[NP];
 #pragma unroll
     for (int q = 0; q < NP; ++q) now[q] = next[q];
-    if (j + 1 < S::TN) ask(j + 1);
-    float v[NP][8];
+    if (ahead && j + 1 < S::TN) {
+#pragma unroll
+      for (int q = 0; q < NP; ++q) next[q] = load16(in, 2 * (in_at + 16 * ldin + 32 * q));
+    }
+    float v[NP][8], w[NP][8];
     take<S>(j, acc, v);
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) pair_up(v[q][r], v[q][4 + r]);
-      float w[8];
-      if (in != nullptr) unpack8(in_type, now[q], w);
-      if constexpr (SLOPE) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[q][i] *= alpha;
-        if (in != nullptr) act_slopes(e.act, w, v[q]);
+      for (int i = 0; i < 8; ++i)
+        v[q][i] = SLOPE ? v[q][i] * alpha : __builtin_fmaf(v[q][i], alpha, each[q][i]);
+    }
+    if constexpr (SLOPE) {
+      if (in != nullptr) {
+        unpack_all<NP>(in_type, now, w);  // aux is never F32 here
+        act_slopes<NP>(e.act, w, v);
+      }
+#pragma unroll
+      for (int q = 0; q < NP; ++q)
 #pragma unroll
         for (int i = 0; i < 8; ++i) each[q][i] += v[q][i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[q][i] = __builtin_fmaf(v[q][i], alpha, each[q][i]);
-        if (e.aux != nullptr) store8(e.aux_type, e.aux, aux0 + 32 * q + 16 * j * e.ldaux, v[q]);
-        act_values(e.act, v[q]);
-        if (in != nullptr) {
-          if (c_exp != 0) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = __builtin_ldexpf(w[i], c_exp);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[q][i] = __builtin_fmaf(beta, w[i], v[q][i]);
-        }
+    } else {
+      if (e.aux != nullptr) {
+        store_all<NP>(e.aux_type, e.aux, aux_at, v);
+        aux_at += 16 * e.ldaux;
       }
-      store8(e.d_type, e.D, d0 + 32 * q + 16 * j * e.ldd, v[q]);
-      if (!SLOPE && e.copy != nullptr)
-        store8(RTAT_TYPE_F16, e.copy, copy0 + 32 * q + 16 * j * e.ldcopy, v[q]);
+      if (e.act != RTAT_ACT_NONE) act_values<NP>(e.act, v);
+      if (in != nullptr) {
+        if (ahead) {
+          unpack_all<NP>(in_type, now, w);
+        } else {
+#pragma unroll
+          for (int q = 0; q < NP; ++q) load8(RTAT_TYPE_F32, in, in_at + 32 * q, w[q]);
+        }
+        if (c_exp != 0) {
+#pragma unroll
+          for (int q = 0; q < NP; ++q)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[q][i] = __builtin_ldexpf(w[q][i], c_exp);
+        }
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[q][i] = __builtin_fmaf(beta, w[q][i], v[q][i]);
+      }
+    }
+    in_at += 16 * ldin;
+    store_all<NP>(e.d_type, e.D, d_at, v);
+    d_at += 16 * e.ldd;
+    if (!SLOPE && e.copy != nullptr) {
+      store_all<NP>(RTAT_TYPE_F16, e.copy, copy_at, v);
+      copy_at += 16 * e.ldcopy;
     }
   }
   if (SLOPE && sums_out != nullptr) {
@@ -302,13 +327,30 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float
       for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int d = 1; d < 16; d *= 2) each[q][i] += __shfl_xor(each[q][i], d);
-      if ((lane & 15) == 0)
-        store8(RTAT_TYPE_F32, sums_out, row + 32 * q, each[q]);
+      if ((lane & 15) == 0) store8(RTAT_TYPE_F32, sums_out, row + 32 * q, each[q]);
     }
   }
 }
 
-template <class S>
+// ... whose epilogue is a factor alone and whose result has the operands' type: straight code.
+template <class T, class S, int J = 0>
+__device__ __forceinline__ void finish_plain(float alpha, uint16_t* at, long ldd,
+                                             const f4_t (&acc)[S::TM][S::TN]) {
+  constexpr int NP = S::TM / 2;
+  float v[NP][8];
+  take_one<S, J>(acc, v);
+#pragma unroll
+  for (int q = 0; q < NP; ++q) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) pair_up(v[q][r], v[q][4 + r]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[q][i] *= alpha;
+    store16(at, 64 * q, pack8(Half<T>::id, v[q]));
+  }
+  if constexpr (J + 1 < S::TN) finish_plain<T, S, J + 1>(alpha, at + 16 * ldd, ldd, acc);
+}
+
+template <class T, class S>
 __device__ __forceinline__ void finish_tile(const Gemm16Args& p, unsigned char* lds, int tile_m, int tile_n,
                                    long z, int wave, int lane,
                                    const f4_t (&acc)[S::TM][S::TN]) {
@@ -332,7 +374,12 @@ __device__ __forceinline__ void finish_tile(const Gemm16Args& p, unsigned char* 
   const bool inside = m0 + S::WTM <= e.rows && n0 + S::WTN <= e.cols &&
                       (e.C == nullptr || (m0 + S::WTM <= e.c_rows && n0 + S::WTN <= e.c_cols));
   if (inside) {
-    if (e.slope) finish_inside<S, true>(e, lane, alpha, beta, c_exp, m0, n0, z, sums_out, acc);
+    if (e.plain)
+      finish_plain<T, S>(alpha,
+                         static_cast<uint16_t*>(e.D) + z * e.d_stride + m0 +
+                             16 * ((lane >> 4) & 1) + 8 * (lane >> 5) + (n0 + (lane & 15)) * e.ldd,
+                         e.ldd, acc);
+    else if (e.slope) finish_inside<S, true>(e, lane, alpha, beta, c_exp, m0, n0, z, sums_out, acc);
     else finish_inside<S, false>(e, lane, alpha, beta, c_exp, m0, n0, z, sums_out, acc);
     if (!mirror) return;
   }
@@ -437,7 +484,7 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_kernel(Gemm16Args p) {
     }
     __syncthreads();
   }
-  finish_tile<S>(p, lds, tile_m, tile_n, z, wave, lane, acc);
+  finish_tile<T, S>(p, lds, tile_m, tile_n, z, wave, lane, acc);
 }
 
 // Global -> LDS mover of one whole panel (buffer loads that write LDS): nothing passes through
@@ -619,7 +666,7 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
   }
   mfma_settle();
   __syncthreads();
-  finish_tile<S>(p, lds, tile_m, tile_n, z, wave, lane, acc);
+  finish_tile<T, S>(p, lds, tile_m, tile_n, z, wave, lane, acc);
 #endif
 }
 
@@ -720,6 +767,9 @@ rtat_status_t launch_gemm16(rtat_native_handle* h, const Gemm16& g) {
   p.ldb = g.ldb;
   p.b_stride = g.b_stride;
   p.ep = g.ep;
+  const Epilogue& e = g.ep;
+  p.ep.plain = !e.slope && e.act == RTAT_ACT_NONE && e.bias == nullptr && e.aux == nullptr &&
+               e.C == nullptr && e.copy == nullptr && e.d_type == g.type;
   return g.type == RTAT_TYPE_BF16 ? launch_type<__bf16>(h, g, p) : launch_type<_Float16>(h, g, p);
 }
 

@@ -39,15 +39,15 @@ __global__ __launch_bounds__(256) void act_backward_kernel(ActArgs p) {
     if (row + 8 <= p.m) {
 #pragma unroll 4
       for (int col = first + lc; col < last; col += COLS) {
-        float v[8], z[8];
-        load8(p.type, p.dD, row + (long)col * p.lddd, v);
+        float v[1][8], z[1][8];
+        load8(p.type, p.dD, row + (long)col * p.lddd, v[0]);
         if (slope) {
-          load8(p.type, p.Z, row + (long)col * p.ldz, z);
+          load8(p.type, p.Z, row + (long)col * p.ldz, z[0]);
           act_slopes(p.act, z, v);
-          if (p.dZ != nullptr) store8(p.type, p.dZ, row + (long)col * p.lddz, v);
+          if (p.dZ != nullptr) store8(p.type, p.dZ, row + (long)col * p.lddz, v[0]);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sums[i] += v[i];
+        for (int i = 0; i < 8; ++i) sums[i] += v[0][i];
       }
     } else {
       for (int col = first + lc; col < last; col += COLS) {
