@@ -43,11 +43,24 @@ template <> struct Half<_Float16> {
 // mfma_into keeps the accumulator in the accumulation registers and its place in the program: a
 // wave that holds 256 of them leaves the compiler no room to move them about, which it otherwise
 // does every iteration.  The compiler does not see a matrix instruction there, so nothing but
-// mfma_into may touch the accumulators until mfma_settle has passed.
-__device__ inline void mfma_settle() {
+// mfma_into may touch the accumulators until mfma_settle has passed: it waits longer than any
+// matrix instruction takes, and hands every accumulator on as a new value, so that no read can
+// move in front of it.
+template <int M, int N>
+__device__ __forceinline__ void mfma_settle(f4_t (&acc)[M][N]) {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < M; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) asm volatile("" : "+a"(acc[i][j]));
   __builtin_amdgcn_sched_barrier(0);
+}
+// An accumulator of mfma_into, after mfma_settle.
+__device__ __forceinline__ float mfma_get(float a) {
+  float v;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(a));
+  return v;
 }
 
 // Sixteen bytes at an address that is only element-aligned (one global load: the hardware
@@ -191,17 +204,6 @@ __device__ inline void store8(int type, void* p, long i, const float (&v)[8]) {
   }
 }
 
-// N times eight 16-bit elements; one choice of type for all.
-template <int N>
-__device__ inline void unpack_all(int type, const u4_t (&r)[N], float (&v)[N][8]) {
-  if (type == RTAT_TYPE_BF16) {
-#pragma unroll
-    for (int q = 0; q < N; ++q) unpack8(RTAT_TYPE_BF16, r[q], v[q]);
-  } else {
-#pragma unroll
-    for (int q = 0; q < N; ++q) unpack8(RTAT_TYPE_F16, r[q], v[q]);
-  }
-}
 // N times eight elements, 32 apart, from element i on.
 template <int N>
 __device__ inline void store_all(int type, void* p, long i, const float (&v)[N][8]) {
@@ -218,13 +220,16 @@ __device__ inline void store_all(int type, void* p, long i, const float (&v)[N][
 }
 
 // N times eight elements through an activation; the choice is made once for all of them.
+// Eight at a time are enough to fill the pipe; all at once would not fit the registers.
 template <int N>
 __device__ inline void act_values(int act, float (&v)[N][8]) {
 #define RTAT_EACH(A)                                     \
   case A:                                                \
-    _Pragma("unroll") for (int q = 0; q < N; ++q)        \
+    _Pragma("unroll") for (int q = 0; q < N; ++q) {      \
       _Pragma("unroll") for (int i = 0; i < 8; ++i)      \
         v[q][i] = act_value(A, v[q][i]);                 \
+      __builtin_amdgcn_sched_barrier(0);                 \
+    }                                                    \
     break;
   switch (act) {
     RTAT_EACH(RTAT_ACT_RELU)
@@ -235,14 +240,18 @@ __device__ inline void act_values(int act, float (&v)[N][8]) {
   }
 #undef RTAT_EACH
 }
-// v *= act'(z)
+// v *= act'(z), z as the 16-bit values in `raw`.
 template <int N>
-__device__ inline void act_slopes(int act, const float (&z)[N][8], float (&v)[N][8]) {
+__device__ inline void act_slopes(int act, int type, const u4_t (&raw)[N], float (&v)[N][8]) {
 #define RTAT_EACH(A)                                     \
   case A:                                                \
-    _Pragma("unroll") for (int q = 0; q < N; ++q)        \
+    _Pragma("unroll") for (int q = 0; q < N; ++q) {      \
+      float z[8];                                        \
+      unpack8(type, raw[q], z);                          \
       _Pragma("unroll") for (int i = 0; i < 8; ++i)      \
-        v[q][i] *= act_slope(A, z[q][i]);                \
+        v[q][i] *= act_slope(A, z[i]);                   \
+      __builtin_amdgcn_sched_barrier(0);                 \
+    }                                                    \
     break;
   switch (act) {
     RTAT_EACH(RTAT_ACT_RELU)
@@ -252,6 +261,23 @@ __device__ inline void act_slopes(int act, const float (&z)[N][8], float (&v)[N]
     default: break;
   }
 #undef RTAT_EACH
+}
+// v += factor * 2^exp * c, c as the 16-bit values in `raw`.
+template <int N>
+__device__ inline void add_scaled(int type, const u4_t (&raw)[N], float factor, int exp,
+                                  float (&v)[N][8]) {
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    float c[8];
+    unpack8(type, raw[q], c);
+    if (exp != 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = __builtin_ldexpf(c[i], exp);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[q][i] = __builtin_fmaf(factor, c[i], v[q][i]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 // What becomes of the product.  Elements (row, col) with row < rows and col < cols are stored.
@@ -298,17 +324,17 @@ __device__ inline void epilogue8(const Epilogue& e, float alpha, float beta, int
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] *= alpha;
   if (row + 8 <= e.rows && (e.C == nullptr || row + 8 <= e.c_rows)) {
-    float w[8];
     if (e.slope) {
       if (e.act != RTAT_ACT_NONE) {
-        load8(e.aux_type, e.aux, aux_at, w);
-        act_slopes<1>(e.act, reinterpret_cast<const float(&)[1][8]>(w), reinterpret_cast<float(&)[1][8]>(v));
+        const u4_t z[1] = {load16(e.aux, 2 * aux_at)};
+        act_slopes<1>(e.act, e.aux_type, z, reinterpret_cast<float(&)[1][8]>(v));
       }
     } else {
       float c[8];
       const bool with_c = e.C != nullptr && col < e.c_cols;
       if (with_c) load8(e.c_type, e.C, c_at, c);
       if (e.bias != nullptr) {
+        float w[8];
         load8(e.bias_type, e.bias, row, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += w[i];

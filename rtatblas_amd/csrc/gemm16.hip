@@ -40,6 +40,7 @@ constexpr int BK16 = 64;
 template <int BM_, int BN_, int WGM_, int WGN_, int OCC_, bool RING_ = false>
 struct Shape16 {
   static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, OCC = OCC_;
+  static constexpr bool RING = RING_;  // panels in a ring, accumulators of mfma_into
   static constexpr int NW = WGM * WGN, NT = 64 * NW;
   static constexpr int WTM = BM / WGM, WTN = BN / WGN;  // wave tile
   static constexpr int TM = WTM / 16, TN = WTN / 16;    // MFMA blocks per wave tile
@@ -173,8 +174,13 @@ struct Parked {
     if (j == J) {
       turn();
 #pragma unroll
-      for (int i = 0; i < S::TM; ++i)
-        *reinterpret_cast<f4_t*>(park + (lane & 15) * S::PARK + 16 * i + 4 * (lane >> 4)) = acc[i][J];
+      for (int i = 0; i < S::TM; ++i) {
+        f4_t v = acc[i][J];
+        if constexpr (S::RING)
+          v = f4_t{mfma_get(acc[i][J][0]), mfma_get(acc[i][J][1]), mfma_get(acc[i][J][2]),
+                   mfma_get(acc[i][J][3])};
+        *reinterpret_cast<f4_t*>(park + (lane & 15) * S::PARK + 16 * i + 4 * (lane >> 4)) = v;
+      }
       turn();
     } else if constexpr (J + 1 < S::TN) {
       put<J + 1>(j, acc);
@@ -214,8 +220,13 @@ __device__ __forceinline__ void take_one(const f4_t (&acc)[S::TM][S::TN], float 
   for (int q = 0; q < S::TM / 2; ++q)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      v[q][r] = acc[2 * q][J][r];
-      v[q][4 + r] = acc[2 * q + 1][J][r];
+      if constexpr (S::RING) {
+        v[q][r] = mfma_get(acc[2 * q][J][r]);
+        v[q][4 + r] = mfma_get(acc[2 * q + 1][J][r]);
+      } else {
+        v[q][r] = acc[2 * q][J][r];
+        v[q][4 + r] = acc[2 * q + 1][J][r];
+      }
     }
   asm volatile("; block column %0" : : "n"(J));  // keeps the compiler from merging the copies of this
 }
@@ -233,7 +244,7 @@ __device__ __forceinline__ void take(int j, const f4_t (&acc)[S::TM][S::TN],
 // accumulators stay in registers: a store instruction covers 64 neighbouring bytes of 16 columns.
 // A wave of the largest tile is alone on its SIMD and waits out every taken branch, so choices
 // are made once per block column.
-template <class S, bool SLOPE>
+template <class T, class S, bool SLOPE>
 __device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float alpha, float beta,
                                               int c_exp, int m0, int n0, long z, float* sums_out,
                                               const f4_t (&acc)[S::TM][S::TN]) {
@@ -267,7 +278,7 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float
 #pragma unroll
       for (int q = 0; q < NP; ++q) next[q] = load16(in, 2 * (in_at + 16 * ldin + 32 * q));
     }
-    float v[NP][8], w[NP][8];
+    float v[NP][8];
     take<S>(j, acc, v);
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
@@ -278,37 +289,32 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float
         v[q][i] = SLOPE ? v[q][i] * alpha : __builtin_fmaf(v[q][i], alpha, each[q][i]);
     }
     if constexpr (SLOPE) {
-      if (in != nullptr) {
-        unpack_all<NP>(in_type, now, w);  // aux is never F32 here
-        act_slopes<NP>(e.act, w, v);
-      }
+      if (in != nullptr) act_slopes<NP>(e.act, Half<T>::id, now, v);
 #pragma unroll
       for (int q = 0; q < NP; ++q)
 #pragma unroll
         for (int i = 0; i < 8; ++i) each[q][i] += v[q][i];
     } else {
       if (e.aux != nullptr) {
-        store_all<NP>(e.aux_type, e.aux, aux_at, v);
+        store_all<NP>(Half<T>::id, e.aux, aux_at, v);
         aux_at += 16 * e.ldaux;
       }
       if (e.act != RTAT_ACT_NONE) act_values<NP>(e.act, v);
       if (in != nullptr) {
-        if (ahead) {
-          unpack_all<NP>(in_type, now, w);
-        } else {
+        if (!ahead) {
 #pragma unroll
-          for (int q = 0; q < NP; ++q) load8(RTAT_TYPE_F32, in, in_at + 32 * q, w[q]);
+          for (int q = 0; q < NP; ++q) {
+            float c[8];
+            load8(RTAT_TYPE_F32, in, in_at + 32 * q, c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              v[q][i] = __builtin_fmaf(beta, __builtin_ldexpf(c[i], c_exp), v[q][i]);
+          }
+        } else if (in_type == Half<T>::id) {
+          add_scaled<NP>(Half<T>::id, now, beta, c_exp, v);
+        } else {  // an f16 product that adds to bf16
+          add_scaled<NP>(RTAT_TYPE_BF16, now, beta, c_exp, v);
         }
-        if (c_exp != 0) {
-#pragma unroll
-          for (int q = 0; q < NP; ++q)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[q][i] = __builtin_ldexpf(w[q][i], c_exp);
-        }
-#pragma unroll
-        for (int q = 0; q < NP; ++q)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[q][i] = __builtin_fmaf(beta, w[q][i], v[q][i]);
       }
     }
     in_at += 16 * ldin;
@@ -347,6 +353,7 @@ __device__ __forceinline__ void finish_plain(float alpha, uint16_t* at, long ldd
     for (int i = 0; i < 8; ++i) v[q][i] *= alpha;
     store16(at, 64 * q, pack8(Half<T>::id, v[q]));
   }
+  __builtin_amdgcn_sched_barrier(0);  // one block column in flight: registers
   if constexpr (J + 1 < S::TN) finish_plain<T, S, J + 1>(alpha, at + 16 * ldd, ldd, acc);
 }
 
@@ -379,8 +386,8 @@ __device__ __forceinline__ void finish_tile(const Gemm16Args& p, unsigned char* 
                          static_cast<uint16_t*>(e.D) + z * e.d_stride + m0 +
                              16 * ((lane >> 4) & 1) + 8 * (lane >> 5) + (n0 + (lane & 15)) * e.ldd,
                          e.ldd, acc);
-    else if (e.slope) finish_inside<S, true>(e, lane, alpha, beta, c_exp, m0, n0, z, sums_out, acc);
-    else finish_inside<S, false>(e, lane, alpha, beta, c_exp, m0, n0, z, sums_out, acc);
+    else if (e.slope) finish_inside<T, S, true>(e, lane, alpha, beta, c_exp, m0, n0, z, sums_out, acc);
+    else finish_inside<T, S, false>(e, lane, alpha, beta, c_exp, m0, n0, z, sums_out, acc);
     if (!mirror) return;
   }
   const Parked<S> k(lds, wave, lane);
@@ -664,7 +671,7 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
     if (kt + 2 < panels) issue_all(kt + 2);
     multiply(1, [&](int x) { read(a1, b1, 0, x); }, no_load);  // of the last panel: not used
   }
-  mfma_settle();
+  mfma_settle(acc);
   __syncthreads();
   finish_tile<T, S>(p, lds, tile_m, tile_n, z, wave, lane, acc);
 #endif

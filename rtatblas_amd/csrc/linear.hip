@@ -39,11 +39,11 @@ __global__ __launch_bounds__(256) void act_backward_kernel(ActArgs p) {
     if (row + 8 <= p.m) {
 #pragma unroll 4
       for (int col = first + lc; col < last; col += COLS) {
-        float v[1][8], z[1][8];
+        float v[1][8];
         load8(p.type, p.dD, row + (long)col * p.lddd, v[0]);
         if (slope) {
-          load8(p.type, p.Z, row + (long)col * p.ldz, z[0]);
-          act_slopes(p.act, z, v);
+          const u4_t z[1] = {load16(p.Z, 2 * (row + (long)col * p.ldz))};
+          act_slopes<1>(p.act, p.type, z, v);
           if (p.dZ != nullptr) store8(p.type, p.dZ, row + (long)col * p.lddz, v[0]);
         }
 #pragma unroll
