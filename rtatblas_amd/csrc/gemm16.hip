@@ -625,29 +625,35 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
     else fb[step][x - 1] = rb.read(pb, x - 1, step);
   };
   // The MFMAs of one K-step, with read(x), x = 0 .. TM + TN - 1, spread behind the first three
-  // quarters of them and load(i), i = 0 .. 7, behind all.
+  // quarters of them (as far as there are enough) and load(i), i = 0 .. NLOAD - 1, behind all.
+  constexpr int NLOAD = decltype(da)::NI;
+  static_assert(NLOAD == decltype(db)::NI && NLOAD <= TM * TN, "a load per MFMA at most");
   auto multiply = [&](int step, auto read_x, auto load_i) {
-    constexpr int NMFMA = TM * TN, GAP = 3 * NMFMA / (4 * (TM + TN)), LOAD_GAP = NMFMA / 8;
+    constexpr int NMFMA = TM * TN, NREAD = TM + TN;
+    constexpr int GAP = 3 * NMFMA >= 4 * NREAD ? 3 * NMFMA / (4 * NREAD) : 1;  // MFMAs to a read
+    constexpr int PER = GAP * NREAD <= NMFMA ? 1 : (NREAD + NMFMA - 1) / NMFMA;  // reads at a time
+    constexpr int LOAD_GAP = NMFMA / NLOAD > 0 ? NMFMA / NLOAD : 1;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         const int x = i * TN + j;
         Half<T>::mfma_into(acc[i][j], fa[step][i], fb[step][j]);
-        if (x % GAP == 0 && x / GAP < TM + TN) {
-          read_x(x / GAP);
+        if (x % GAP == 0 && x / GAP * PER < NREAD) {
+#pragma unroll
+          for (int y = 0; y < PER; ++y)
+            if (x / GAP * PER + y < NREAD) read_x(x / GAP * PER + y);
           __builtin_amdgcn_sched_barrier(0);
         }
-        if (x % LOAD_GAP == LOAD_GAP / 2) load_i(x / LOAD_GAP);
+        if (x % LOAD_GAP == LOAD_GAP / 2 && x / LOAD_GAP < NLOAD) load_i(x / LOAD_GAP);
       }
   };
-  static_assert(decltype(da)::NI == 8 && decltype(db)::NI == 8, "eight loads a panel");
   auto no_load = [](int) {};
 
   if (panels > 0) {
     issue_all(0);
     if (panels > 1) issue_all(1);
-    if (whole > 1) wait_and_meet<16>();
+    if (whole > 1) wait_and_meet<2 * NLOAD>();
     else wait_and_meet<0>();
 #pragma unroll
     for (int x = 0; x < TM + TN; ++x) read(slot(0), slot(1), 0, x);
@@ -659,7 +665,7 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
     const u4_t pa = da.panel_at(At, p.lda, kt + 2), pb = db.panel_at(Bt, p.ldb, kt + 2);
     const unsigned to_a = lds_address(slot(2 * kt + 4)), to_b = lds_address(a0);
     multiply(0, [&](int x) { read(a0, b0, 1, x); }, [&](int i) { da.issue(i, pa, to_a, wave); });
-    wait_and_meet<8>();
+    wait_and_meet<NLOAD>();
     multiply(1, [&](int x) { read(a1, b1, 0, x); }, [&](int i) { db.issue(i, pb, to_b, wave); });
   }
 #pragma unroll 1
@@ -678,7 +684,9 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
 }
 
 typedef Shape16<256, 256, 2, 2, 1, true> S256x256;  // loads straight to LDS
-typedef Shape16<128, 128, 2, 2, 2> S128x128;
+typedef Shape16<128, 128, 2, 2, 2, true> R128x128;
+typedef Shape16<64, 64, 2, 2, 4, true> R64x64;
+typedef Shape16<128, 128, 2, 2, 2> S128x128;  // any alignment
 typedef Shape16<64, 64, 2, 2, 4> S64x64;
 
 template <class S>
@@ -734,6 +742,8 @@ rtat_status_t launch_type(rtat_native_handle* h, const Gemm16& g, const Gemm16Ar
   };
   if (direct(p.A, p.lda, p.a_stride) && direct(p.B, p.ldb, p.b_stride)) {
     if (tiles(256) >= cus / 2) return launch_ops16<T, S256x256, true>(h, g, p);
+    if (tiles(128) >= cus) return launch_ops16<T, R128x128, true>(h, g, p);
+    return launch_ops16<T, R64x64, true>(h, g, p);
   }
   if (tiles(128) >= cus) return launch_ops16<T, S128x128, false>(h, g, p);
   return launch_ops16<T, S64x64, false>(h, g, p);
