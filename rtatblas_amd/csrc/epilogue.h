@@ -228,7 +228,7 @@ __device__ inline void act_values(int act, float (&v)[N][8]) {
     _Pragma("unroll") for (int q = 0; q < N; ++q) {      \
       _Pragma("unroll") for (int i = 0; i < 8; ++i)      \
         v[q][i] = act_value(A, v[q][i]);                 \
-      __builtin_amdgcn_sched_barrier(0);                 \
+      if (N > 1) __builtin_amdgcn_sched_barrier(0);      \
     }                                                    \
     break;
   switch (act) {
@@ -250,7 +250,7 @@ __device__ inline void act_slopes(int act, int type, const u4_t (&raw)[N], float
       unpack8(type, raw[q], z);                          \
       _Pragma("unroll") for (int i = 0; i < 8; ++i)      \
         v[q][i] *= act_slope(A, z[i]);                   \
-      __builtin_amdgcn_sched_barrier(0);                 \
+      if (N > 1) __builtin_amdgcn_sched_barrier(0);      \
     }                                                    \
     break;
   switch (act) {

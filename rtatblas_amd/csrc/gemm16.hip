@@ -28,6 +28,9 @@ namespace {
 struct Gemm16Args {
   int m, n, k, tri;
   int tiles_m, tiles_n, tiles;  // tiles per matrix of the batch
+  // slices > 1 (batch 1 only): each tile is computed by that many workgroups, one per slice of the
+  // K panels; slice z leaves its raw sums in "matrix" z of D, and join_kernel adds them up.
+  int slices;
   const uint16_t* A;
   long lda, a_stride;
   const uint16_t* B;
@@ -202,6 +205,18 @@ struct Parked {
   }
 };
 
+// Epilogue::scale applied to the factors of matrix z.
+__device__ inline void scale_factors(const Epilogue& e, long z, float& alpha, float& beta,
+                                     int& c_exp) {
+  if (e.scale == nullptr) return;
+  const float r = e.scale[2 * z];
+  for (int i = 0; i < e.r_power; ++i) alpha *= r;
+  if (e.scale_c) {
+    beta *= r;
+    c_exp = (int)e.scale[2 * z + 1];
+  }
+}
+
 // Two accumulators of neighbouring blocks, 16 rows apart, exchanged between neighbouring groups of
 // 16 lanes, so that x and y become the first and second four of eight neighbouring rows of the
 // lane's column: rows 16 (q % 2) + 8 (q / 2) .. + 7 of the pair's 32, q = lane / 16.
@@ -366,18 +381,12 @@ __device__ __forceinline__ void finish_tile(const Gemm16Args& p, unsigned char* 
   const int n0 = tile_n * S::BN + (wave / S::WGM) * S::WTN;
   float alpha = e.alpha, beta = e.beta;
   int c_exp = 0;
-  if (e.scale != nullptr) {
-    const float r = e.scale[2 * z];
-    for (int i = 0; i < e.r_power; ++i) alpha *= r;
-    if (e.scale_c) {
-      beta *= r;
-      c_exp = (int)e.scale[2 * z + 1];
-    }
-  }
+  scale_factors(e, z, alpha, beta, c_exp);
   // One row of partial sums per wave column.
   float* sums_out =
       e.sums != nullptr ? e.sums + (long)(tile_n * S::WGN + wave / S::WGM) * e.rows : nullptr;
-  const bool mirror = p.tri != 0 && tile_m != tile_n;
+  // The slices of a triangular product are mirrored when they are joined.
+  const bool mirror = p.tri != 0 && tile_m != tile_n && p.slices == 1;
   const bool inside = m0 + S::WTM <= e.rows && n0 + S::WTN <= e.cols &&
                       (e.C == nullptr || (m0 + S::WTM <= e.c_rows && n0 + S::WTN <= e.c_cols));
   if (inside) {
@@ -431,6 +440,23 @@ __device__ __forceinline__ void finish_tile(const Gemm16Args& p, unsigned char* 
   }
 }
 
+// The K range of matrix (or slice) z, and an operand's first element in it.
+__device__ inline void k_range(const Gemm16Args& p, long z, int& first, int& len) {
+  first = 0;
+  len = p.k;
+  if (p.slices > 1) {  // panels [z n / slices, (z + 1) n / slices) of the n K panels
+    const long n = (p.k + BK16 - 1) / BK16;
+    first = (int)(z * n / p.slices) * BK16;
+    const int end = (int)((z + 1) * n / p.slices) * BK16;
+    len = (end < p.k ? end : p.k) - first;
+  }
+}
+template <bool KMAJOR>
+__device__ inline const uint16_t* first_k(const uint16_t* base, long ld, long stride, int slices,
+                                          long z, int k) {
+  return (slices > 1 ? base : base + z * stride) + (KMAJOR ? (long)k : (long)k * ld);
+}
+
 template <class T, class S, bool KA, bool KB>
 __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_kernel(Gemm16Args p) {
   constexpr int TM = S::TM, TN = S::TN;
@@ -443,8 +469,10 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_kernel(Gemm16Args p) {
   int tile_m, tile_n;
   tile_of_logical(logical % p.tiles, p.tiles_m, p.tiles_n, p.tri, S::BM, S::BN, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::BN;
-  const uint16_t* A = p.A + z * p.a_stride;
-  const uint16_t* B = p.B + z * p.b_stride;
+  int k_first, k_len;
+  k_range(p, z, k_first, k_len);
+  const uint16_t* A = first_k<KA>(p.A, p.lda, p.a_stride, p.slices, z, k_first);
+  const uint16_t* B = first_k<KB>(p.B, p.ldb, p.b_stride, p.slices, z, k_first);
 
   f4_t acc[TM][TN];
 #pragma unroll
@@ -452,15 +480,15 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_kernel(Gemm16Args p) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{0, 0, 0, 0};
 
-  const int panels = (p.k + BK16 - 1) / BK16;
+  const int panels = (k_len + BK16 - 1) / BK16;
   typedef Panel16<KA, S::BM> PA;
   const Frags16<KA, S::BM> ra(wm0, lane);
   const Frags16<KB, S::BN> rb(wn0, lane);
   Mover16<KA, S::BM, S::NT> ma;
   Mover16<KB, S::BN, S::NT> mb;
   auto load = [&](int kt) {
-    ma.load(A, p.lda, m0, p.m, kt * BK16, p.k, t);
-    mb.load(B, p.ldb, n0, p.n, kt * BK16, p.k, t);
+    ma.load(A, p.lda, m0, p.m, kt * BK16, k_len, t);
+    mb.load(B, p.ldb, n0, p.n, kt * BK16, k_len, t);
   };
   auto store = [&](int kt) {
     unsigned char* stage = lds + (kt & 1) * S::STAGE;
@@ -573,8 +601,10 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
   int tile_m, tile_n;
   tile_of_logical(logical % p.tiles, p.tiles_m, p.tiles_n, p.tri, S::BM, S::BN, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::BN;
-  const uint16_t* A = p.A + z * p.a_stride;
-  const uint16_t* B = p.B + z * p.b_stride;
+  int k_first, k_len;
+  k_range(p, z, k_first, k_len);
+  const uint16_t* A = first_k<KA>(p.A, p.lda, p.a_stride, p.slices, z, k_first);
+  const uint16_t* B = first_k<KB>(p.B, p.ldb, p.b_stride, p.slices, z, k_first);
   const uint16_t* At = A + (KA ? (long)m0 * p.lda : (long)m0);
   const uint16_t* Bt = B + (KB ? (long)n0 * p.ldb : (long)n0);
 
@@ -590,8 +620,10 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
   da.init(p.lda, m0, p.m, wave, lane);
   db.init(p.ldb, n0, p.n, wave, lane);
   // Panels 0 .. whole - 1 go straight to LDS; a last one may need guards.
-  const int panels = (p.k + BK16 - 1) / BK16;
-  const bool ragged = p.k % BK16 != 0 || (!KA && m0 + S::BM > p.m) || (!KB && n0 + S::BN > p.n);
+  const int panels = (k_len + BK16 - 1) / BK16;
+  const bool ragged = k_len % BK16 != 0 ||
+                      (k_first + k_len == p.k &&
+                       ((!KA && m0 + S::BM > p.m) || (!KB && n0 + S::BN > p.n)));
   const int whole = panels - (ragged ? 1 : 0);
   // Item 2 kt is A of panel kt, item 2 kt + 1 its B; item x lies in slot x % 5.
   static_assert(S::BM == S::BN && S::LDS >= 5 * PA::BYTES, "slots of one size");
@@ -607,11 +639,11 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
     } else {
       {
         Mover16<KA, S::BM, S::NT> ma;
-        ma.load(A, p.lda, m0, p.m, kt * BK16, p.k, t);
+        ma.load(A, p.lda, m0, p.m, kt * BK16, k_len, t);
         ma.store(slot(2 * kt), t);
       }
       Mover16<KB, S::BN, S::NT> mb;
-      mb.load(B, p.ldb, n0, p.n, kt * BK16, p.k, t);
+      mb.load(B, p.ldb, n0, p.n, kt * BK16, k_len, t);
       mb.store(slot(2 * kt + 1), t);
     }
   };
@@ -689,6 +721,69 @@ typedef Shape16<64, 64, 2, 2, 4, true> R64x64;
 typedef Shape16<128, 128, 2, 2, 2> S128x128;  // any alignment
 typedef Shape16<64, 64, 2, 2, 4> S64x64;
 
+// Sums of the slices of a split product, in order, and their epilogue.
+constexpr int JOIN_ROWS = 128, JOIN_COLS = 16;  // of C per workgroup
+struct JoinArgs {
+  Epilogue ep;
+  const float* parts;  // slice z: columns of ldp floats, ep.cols of them
+  long ldp;
+  int slices, tri;
+};
+inline long slice_ld(int m) { return ((long)m + 7) / 8 * 8; }
+
+__global__ __launch_bounds__(256) void join_kernel(JoinArgs p) {
+  __shared__ float part[JOIN_COLS][JOIN_ROWS];
+  const int t = threadIdx.x, lr = (t % 16) * 8, lc = t / 16;
+  const int row = blockIdx.x * JOIN_ROWS + lr, col = blockIdx.y * JOIN_COLS + lc;
+  const Epilogue& e = p.ep;
+  // A triangular product leaves the tiles on and below the diagonal.
+  if (p.tri != 0 && blockIdx.x < blockIdx.y * JOIN_COLS / JOIN_ROWS) return;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+  if (row < e.rows && col < e.cols) {
+    const float* at = p.parts + row + (long)col * p.ldp;
+    const long step = p.ldp * e.cols;
+#pragma unroll 4
+    for (int z = 0; z < p.slices; ++z) {
+      const f4_t* q = reinterpret_cast<const f4_t*>(at + z * step);
+      const f4_t lo = q[0], hi = q[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] += lo[i];
+        v[4 + i] += hi[i];
+      }
+    }
+  }
+  float alpha = e.alpha, beta = e.beta;
+  int c_exp = 0;
+  scale_factors(e, 0, alpha, beta, c_exp);
+  const bool mirror = p.tri != 0 && blockIdx.x != blockIdx.y * JOIN_COLS / JOIN_ROWS;
+  if (mirror || e.sums != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[lc][lr + i] = v[i];
+  }
+  epilogue8(e, alpha, beta, c_exp, row, col, 0, v);
+  if (mirror) {
+    // The same values as sixteen rows of the mirrored columns.
+    __syncthreads();
+    const int r = t >> 1, c = 8 * (t & 1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = part[c + i][r];
+    epilogue8(e, alpha, beta, c_exp, blockIdx.y * JOIN_COLS + c, blockIdx.x * JOIN_ROWS + r, 0, v);
+  }
+  if (e.sums == nullptr) return;  // only gradients have them, and those are never triangular
+#pragma unroll
+  for (int i = 0; i < 8; ++i) part[lc][lr + i] = v[i];
+  __syncthreads();
+  if (t < JOIN_ROWS && (int)(blockIdx.x * JOIN_ROWS) + t < e.rows) {
+    float s = 0.0f;
+#pragma unroll
+    for (int c = 0; c < JOIN_COLS; ++c) s += part[c][t];
+    e.sums[(long)blockIdx.y * e.rows + blockIdx.x * JOIN_ROWS + t] = s;
+  }
+}
+
 template <class S>
 rtat_status_t launch_kernel(rtat_native_handle* h, const Gemm16& g, Gemm16Args p,
                             void (*kern)(Gemm16Args), PerDeviceOnce& configured) {
@@ -704,10 +799,37 @@ rtat_status_t launch_kernel(rtat_native_handle* h, const Gemm16& g, Gemm16Args p
   p.tiles_m = (p.m + S::BM - 1) / S::BM;
   p.tiles_n = (p.n + S::BN - 1) / S::BN;
   const long tiles = p.tri != 0 ? (long)p.tiles_m * (p.tiles_m + 1) / 2 : (long)p.tiles_m * p.tiles_n;
-  if (tiles * g.batch > 0x7fffffffL) return RTAT_STATUS_INVALID_VALUE;
+  const long count = tiles * (p.slices > 1 ? p.slices : g.batch);
+  if (count > 0x7fffffffL) return RTAT_STATUS_INVALID_VALUE;
   p.tiles = (int)tiles;
   h->sum_rows = p.tiles_n * S::WGN;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(tiles * g.batch)), dim3(S::NT), S::LDS, h->stream, p);
+  if (p.slices == 1) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)count), dim3(S::NT), S::LDS, h->stream, p);
+    return launch_status();
+  }
+  JoinArgs j = {};
+  j.ep = p.ep;
+  j.parts = static_cast<const float*>(h->split_ws);
+  j.ldp = slice_ld(p.m);
+  j.slices = p.slices;
+  j.tri = p.tri;
+  Epilogue raw = {};
+  raw.rows = raw.c_rows = p.m;
+  raw.cols = raw.c_cols = p.n;
+  raw.alpha = 1.0f;
+  raw.D = h->split_ws;
+  raw.ldd = j.ldp;
+  raw.d_stride = j.ldp * p.n;
+  raw.d_type = RTAT_TYPE_F32;
+  p.ep = raw;
+  hipLaunchKernelGGL(kern, dim3((unsigned)count), dim3(S::NT), S::LDS, h->stream, p);
+  const rtat_status_t st = launch_status();
+  if (st != RTAT_STATUS_SUCCESS) return st;
+  static_assert(JOIN_ROWS % JOIN_COLS == 0, "a block of the join lies in one tile row and column");
+  const dim3 grid((unsigned)((p.m + JOIN_ROWS - 1) / JOIN_ROWS),
+                  (unsigned)((p.n + JOIN_COLS - 1) / JOIN_COLS));
+  h->sum_rows = (int)grid.y;
+  hipLaunchKernelGGL(join_kernel, grid, dim3(256), 0, h->stream, j);
   return launch_status();
 }
 
@@ -734,19 +856,53 @@ bool direct(const void* base, long ld, long stride) {
          ld < (1L << 23);
 }
 
+// Slices for `tiles` tiles on `slots` workgroup slots, at most as many as fill the slots once, each
+// of at least MIN_SLICE panels, that fit the handle's slice scratch: the number with the shortest
+// estimate.  `panel_us`: what a panel of a lone tile takes; the second launch takes 5 us, slices
+// are written and read once at 3 MB/us.  (512 x 512 x 8192 46 -> 19 us, 8192 x 1 x 2048 14 -> 11 us;
+// 1024^3, left whole, takes 7.7 us and would take 16.9 in two.)
+constexpr int MIN_SLICE = 4;
+int slices_for(const rtat_native_handle* h, const Gemm16& g, long tiles, long slots,
+               double panel_us, double& shortest) {
+  const long panels = (g.k + BK16 - 1) / BK16;
+  const long each = slice_ld(g.m) * g.n * 4;
+  shortest = panel_us * (double)panels;
+  if (g.batch != 1 || h->user_ws != nullptr || h->split_ws == nullptr) return 1;
+  long most = slots / tiles;
+  if (most > panels / MIN_SLICE) most = panels / MIN_SLICE;
+  if (most > (long)SPLIT_WS_BYTES / each) most = (long)SPLIT_WS_BYTES / each;
+  int best = 1;
+  for (long s = 2; s <= most; ++s) {
+    const double moved = (double)(2 * s * each) * (g.tri ? 0.5 : 1.0);
+    const double us = panel_us * (double)panels / (double)s + 5.0 + moved / 3e6;
+    if (us < shortest) {
+      shortest = us;
+      best = (int)s;
+    }
+  }
+  return best;
+}
+
 template <class T>
-rtat_status_t launch_type(rtat_native_handle* h, const Gemm16& g, const Gemm16Args& p) {
+rtat_status_t launch_type(rtat_native_handle* h, const Gemm16& g, Gemm16Args p) {
   const long cus = h->compute_units > 0 ? h->compute_units : 256;
   auto tiles = [&](int b) {
-    return (long)((p.m + b - 1) / b) * ((p.n + b - 1) / b) * g.batch / (p.tri ? 2 : 1);
+    const long tm = (p.m + b - 1) / b, tn = (p.n + b - 1) / b;
+    return (p.tri ? tm * (tm + 1) / 2 : tm * tn) * g.batch;
   };
-  if (direct(p.A, p.lda, p.a_stride) && direct(p.B, p.ldb, p.b_stride)) {
-    if (tiles(256) >= cus / 2) return launch_ops16<T, S256x256, true>(h, g, p);
-    if (tiles(128) >= cus) return launch_ops16<T, R128x128, true>(h, g, p);
-    return launch_ops16<T, R64x64, true>(h, g, p);
+  const bool ring = direct(p.A, p.lda, p.a_stride) && direct(p.B, p.ldb, p.b_stride);
+  if (ring && tiles(256) >= cus / 2) return launch_ops16<T, S256x256, true>(h, g, p);
+  bool large = tiles(128) >= cus;
+  double us;
+  if (!large && p.tri != 0) {
+    // A symmetric product's slices are joined in blocks of the 128 x 128 tile.
+    large = tiles(128) * 2 >= cus;
+    if (large) p.slices = slices_for(h, g, tiles(128), 2 * cus, 0.55, us);
   }
-  if (tiles(128) >= cus) return launch_ops16<T, S128x128, false>(h, g, p);
-  return launch_ops16<T, S64x64, false>(h, g, p);
+  if (large)
+    return ring ? launch_ops16<T, R128x128, true>(h, g, p) : launch_ops16<T, S128x128, false>(h, g, p);
+  if (p.tri == 0) p.slices = slices_for(h, g, tiles(64), 2 * cus, 0.3, us);
+  return ring ? launch_ops16<T, R64x64, true>(h, g, p) : launch_ops16<T, S64x64, false>(h, g, p);
 }
 
 __global__ __launch_bounds__(256) void sum_rows_kernel(const float* parts, int count, int m,
@@ -761,7 +917,7 @@ __global__ __launch_bounds__(256) void sum_rows_kernel(const float* parts, int c
 
 }  // namespace
 
-int dact_sum_rows(int n) { return 2 * ((n + 63) / 64); }
+int dact_sum_rows(int n) { return 4 * ((n + 63) / 64); }
 
 rtat_status_t launch_sum_rows(rtat_native_handle* h, const float* parts, int count, int m,
                               float* out) {
@@ -777,6 +933,7 @@ rtat_status_t launch_gemm16(rtat_native_handle* h, const Gemm16& g) {
   p.n = g.n;
   p.k = g.k;
   p.tri = g.tri;
+  p.slices = 1;
   p.A = static_cast<const uint16_t*>(g.A);
   p.lda = g.lda;
   p.a_stride = g.a_stride;

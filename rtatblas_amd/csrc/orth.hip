@@ -27,7 +27,7 @@ namespace rtat_native {
 namespace {
 
 constexpr float X_SCALE = 1024.0f, M_SCALE = 1024.0f, P_SCALE = 256.0f;
-constexpr int NORM_BLOCKS = 256;
+constexpr int NORM_BLOCKS = 1024;  // partial sums per matrix, at most
 
 struct NormArgs {
   int type, m, n, mp, np, blocks;
@@ -49,18 +49,30 @@ __device__ inline double block_sum(double s, double* lds) {
   return lds[0] + lds[1] + lds[2] + lds[3];
 }
 
-// Partial sums of squares, a wave per column.
+// Eight rows of a column from `row` on; rows past m read as zero.
+__device__ inline void rows8(const NormArgs& p, long at, int row, float (&v)[8]) {
+  if (row + 8 <= p.m) {
+    load8(p.type, p.G, at + row, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = row + i < p.m ? load_one(p.type, p.G, at + row + i) : 0.0f;
+  }
+}
+
+// Partial sums of squares: a matrix is cut into pieces of eight rows of a column, dealt to the
+// threads of all blocks in turn.
 __global__ __launch_bounds__(256) void norm_kernel(NormArgs p) {
   __shared__ double lds[4];
-  const long z = blockIdx.y;
+  const long z = blockIdx.y, per_col = (p.m + 7) / 8, pieces = per_col * p.n;
+  const long step = 256L * p.blocks;
   double s = 0.0;
-  for (int col = blockIdx.x * 4 + threadIdx.x / 64; col < p.n; col += 4 * p.blocks) {
-    const long at = z * p.stride_g + (long)col * p.ldg;
 #pragma unroll 4
-    for (int row = threadIdx.x % 64; row < p.m; row += 64) {
-      const double x = load_one(p.type, p.G, at + row);
-      s += x * x;
-    }
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < pieces; i += step) {
+    const long col = i / per_col;
+    float v[8];
+    rows8(p, z * p.stride_g + col * p.ldg, (int)(i - col * per_col) * 8, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += (double)v[e] * (double)v[e];
   }
   s = block_sum(s, lds);
   if (threadIdx.x == 0) p.parts[z * p.blocks + blockIdx.x] = s;
@@ -70,7 +82,8 @@ __global__ __launch_bounds__(256) void norm_kernel(NormArgs p) {
 __global__ __launch_bounds__(256) void scale_kernel(NormArgs p) {
   __shared__ double lds[4];
   const long z = blockIdx.y;
-  double s = (int)threadIdx.x < p.blocks ? p.parts[z * p.blocks + threadIdx.x] : 0.0;
+  double s = 0.0;
+  for (int i = threadIdx.x; i < p.blocks; i += 256) s += p.parts[z * p.blocks + i];
   s = block_sum(s, lds);
   const double want = (double)X_SCALE / (sqrt(s) + (double)p.eps);
   // want is 0 or NaN for a G that holds an infinity or a NaN, infinite for a zero norm: the
@@ -87,15 +100,22 @@ __global__ __launch_bounds__(256) void scale_kernel(NormArgs p) {
     p.scale[2 * z] = (float)r;
     p.scale[2 * z + 1] = (float)e;
   }
-  _Float16* X = reinterpret_cast<_Float16*>(p.X) + z * p.x_stride;
-  for (int col = blockIdx.x * 4 + threadIdx.x / 64; col < p.np; col += 4 * gridDim.x) {
-    const long at = z * p.stride_g + (long)col * p.ldg;
+  uint16_t* X = p.X + z * p.x_stride;
+  const long per_col = p.mp / 8, pieces = per_col * p.np, step = 256L * gridDim.x;
 #pragma unroll 4
-    for (int row = threadIdx.x % 64; row < p.mp; row += 64) {
-      const bool in = row < p.m && col < p.n;
-      const float x = in ? load_one(p.type, p.G, at + row) : 0.0f;
-      X[row + (long)col * p.mp] = (_Float16)__builtin_ldexpf(x, e);
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < pieces; i += step) {
+    const long col = i / per_col;
+    const int row = (int)(i - col * per_col) * 8;
+    float v[8];
+    if (col < p.n && row < p.m) {
+      rows8(p, z * p.stride_g + col * p.ldg, row, v);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = 0.0f;
     }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = __builtin_ldexpf(v[q], e);
+    store8(RTAT_TYPE_F16, X, row + col * p.mp, v);
   }
 }
 
@@ -155,7 +175,11 @@ rtat_status_t launch_newton_schulz(rtat_native_handle* h, int g_type, int m, int
   a.n = n;
   a.mp = (int)l.mp;
   a.np = (int)l.np;
-  a.blocks = (n + 3) / 4 < NORM_BLOCKS ? (n + 3) / 4 : NORM_BLOCKS;
+  auto blocks_for = [](long pieces) {  // two pieces a thread
+    const long b = (pieces + 511) / 512;
+    return (int)(b < NORM_BLOCKS ? b : NORM_BLOCKS);
+  };
+  a.blocks = blocks_for((((long)m + 7) / 8) * n);
   a.G = G;
   a.ldg = ldg;
   a.stride_g = stride_g;
@@ -168,8 +192,7 @@ rtat_status_t launch_newton_schulz(rtat_native_handle* h, int g_type, int m, int
                      h->stream, a);
   rtat_status_t st = launch_status();
   if (st != RTAT_STATUS_SUCCESS) return st;
-  const unsigned wgs = (unsigned)((l.np + 3) / 4 < 1024 ? (l.np + 3) / 4 : 1024);
-  hipLaunchKernelGGL(scale_kernel, dim3(wgs, (unsigned)batch), dim3(256), 0, h->stream, a);
+  hipLaunchKernelGGL(scale_kernel, dim3((unsigned)blocks_for(l.mp / 8 * l.np), (unsigned)batch), dim3(256), 0, h->stream, a);
   st = launch_status();
   if (st != RTAT_STATUS_SUCCESS) return st;
 

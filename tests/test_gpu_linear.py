@@ -265,7 +265,8 @@ def test_backward_in_place_and_parts(handle):
 
 @pytest.mark.parametrize("act", range(5))
 @pytest.mark.parametrize("which,pad,size", [("bf16", 0, (512, 300, 128)), ("f16", 1, (131, 70, 65)), ("bf16", 8, (1, 9, 3)),
-                                            ("f16", 0, (264, 1, 40)), ("bf16", 2, (1500, 260, 96))])
+                                            ("f16", 0, (264, 1, 40)), ("bf16", 2, (1500, 260, 96)),
+                                            ("bf16", 0, (300, 20, 1024)), ("f16", 3, (77, 130, 2100))])
 def test_dact(handle, act, which, pad, size):
     import torch
     dt, ty = _types()[which]

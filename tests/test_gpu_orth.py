@@ -58,7 +58,7 @@ def test_shapes(handle, which, kind, m, n):
     _check(src, O, coeffs)
 
 
-@pytest.mark.parametrize("m,n", [(4100, 4200), (4250, 4099)])
+@pytest.mark.parametrize("m,n", [(4100, 4200), (4250, 4099), (2048, 4100), (3000, 1990)])
 def test_large(handle, m, n):
     import torch
     gen = torch.Generator(device="cuda").manual_seed(m)
