@@ -139,8 +139,8 @@ Gemm16 product(int type, bool ta, bool tb, int m, int n, int k, float alpha, con
   g.lda = lda;
   g.B = B;
   g.ldb = ldb;
-  g.ep.rows = g.ep.c_rows = m;
-  g.ep.cols = g.ep.c_cols = n;
+  g.ep.rows = m;
+  g.ep.cols = n;
   g.ep.alpha = alpha;
   g.ep.bias_type = g.ep.aux_type = type;
   return g;

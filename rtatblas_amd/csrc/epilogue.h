@@ -262,18 +262,13 @@ __device__ inline void act_slopes(int act, int type, const u4_t (&raw)[N], float
   }
 #undef RTAT_EACH
 }
-// v += factor * 2^exp * c, c as the 16-bit values in `raw`.
+// v += factor * c, c as the 16-bit values in `raw`.
 template <int N>
-__device__ inline void add_scaled(int type, const u4_t (&raw)[N], float factor, int exp,
-                                  float (&v)[N][8]) {
+__device__ inline void add_scaled(int type, const u4_t (&raw)[N], float factor, float (&v)[N][8]) {
 #pragma unroll
   for (int q = 0; q < N; ++q) {
     float c[8];
     unpack8(type, raw[q], c);
-    if (exp != 0) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = __builtin_ldexpf(c[i], exp);
-    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[q][i] = __builtin_fmaf(factor, c[i], v[q][i]);
     __builtin_amdgcn_sched_barrier(0);
@@ -283,13 +278,13 @@ __device__ inline void add_scaled(int type, const u4_t (&raw)[N], float factor, 
 // What becomes of the product.  Elements (row, col) with row < rows and col < cols are stored.
 //   forward (slope == 0): z = alpha * acc + bias[row]; aux = z; D = act(z) + beta * C
 //   gradient (slope == 1): D = alpha * acc * act'(aux); sums += D along the columns
-// C counts as zero outside c_rows x c_cols.  `copy` receives what D does, in f16.  `scale`, if
-// given, points to a pair (r, e) per matrix of a batch on the device: alpha is multiplied by
-// r^r_power and, when scale_c, C is read as r * 2^e * C.
+// `copy` receives what D does, in f16; `diag` is added to D(i, i).  `scale`, if given, points to a
+// number r per matrix of a batch on the device: alpha is multiplied by r^r_power and, when
+// scale_c, beta by r.
 struct Epilogue {
   int rows, cols;
   int act, slope;
-  float alpha, beta;
+  float alpha, beta, diag;
   const void* bias;
   int bias_type;
   void* aux;
@@ -297,7 +292,7 @@ struct Epilogue {
   int aux_type;
   const void* C;
   long ldc, c_stride;
-  int c_type, c_rows, c_cols;
+  int c_type;
   void* D;
   long ldd, d_stride;
   int d_type;
@@ -309,10 +304,17 @@ struct Epilogue {
   int plain;  // nothing but alpha, and D has the operands' type (set by launch_gemm16)
 };
 
+__device__ inline void add_diagonal(float diag, int row, int col, float (&v)[8]) {
+  if (diag != 0.0f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += row + i == col ? diag : 0.0f;
+  }
+}
+
 // Rows row .. row + 7 of column col, batch matrix z: v holds the accumulators and, for a
 // gradient, leaves with the values that belong to the row sums (0 outside).
-__device__ inline void epilogue8(const Epilogue& e, float alpha, float beta, int c_exp, int row,
-                                 int col, long z, float (&v)[8]) {
+__device__ inline void epilogue8(const Epilogue& e, float alpha, float beta, int row, int col,
+                                 long z, float (&v)[8]) {
   if (col >= e.cols || row >= e.rows) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.0f;
@@ -323,7 +325,7 @@ __device__ inline void epilogue8(const Epilogue& e, float alpha, float beta, int
   const long c_at = z * e.c_stride + row + (long)col * e.ldc;
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] *= alpha;
-  if (row + 8 <= e.rows && (e.C == nullptr || row + 8 <= e.c_rows)) {
+  if (row + 8 <= e.rows) {
     if (e.slope) {
       if (e.act != RTAT_ACT_NONE) {
         const u4_t z[1] = {load16(e.aux, 2 * aux_at)};
@@ -331,7 +333,7 @@ __device__ inline void epilogue8(const Epilogue& e, float alpha, float beta, int
       }
     } else {
       float c[8];
-      const bool with_c = e.C != nullptr && col < e.c_cols;
+      const bool with_c = e.C != nullptr;
       if (with_c) load8(e.c_type, e.C, c_at, c);
       if (e.bias != nullptr) {
         float w[8];
@@ -343,9 +345,10 @@ __device__ inline void epilogue8(const Epilogue& e, float alpha, float beta, int
       act_values<1>(e.act, reinterpret_cast<float(&)[1][8]>(v));
       if (with_c) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(beta, __builtin_ldexpf(c[i], c_exp), v[i]);
+        for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(beta, c[i], v[i]);
       }
     }
+    add_diagonal(e.diag, row, col, v);
     store8(e.d_type, e.D, d_at, v);
     if (e.copy != nullptr)
       store8(RTAT_TYPE_F16, e.copy, z * e.copy_stride + row + (long)col * e.ldcopy, v);
@@ -364,8 +367,8 @@ __device__ inline void epilogue8(const Epilogue& e, float alpha, float beta, int
         if (e.bias != nullptr) x += load_one(e.bias_type, e.bias, row + i);
         if (e.aux != nullptr) store_one(e.aux_type, e.aux, aux_at + i, x);
         x = act_value(e.act, x);
-        if (e.C != nullptr && row + i < e.c_rows && col < e.c_cols)
-          x = __builtin_fmaf(beta, __builtin_ldexpf(load_one(e.c_type, e.C, c_at + i), c_exp), x);
+        if (e.C != nullptr) x = __builtin_fmaf(beta, load_one(e.c_type, e.C, c_at + i), x);
+        if (row + i == col) x += e.diag;
       }
       store_one(e.d_type, e.D, d_at + i, x);
       if (e.copy != nullptr)

@@ -206,15 +206,11 @@ struct Parked {
 };
 
 // Epilogue::scale applied to the factors of matrix z.
-__device__ inline void scale_factors(const Epilogue& e, long z, float& alpha, float& beta,
-                                     int& c_exp) {
+__device__ inline void scale_factors(const Epilogue& e, long z, float& alpha, float& beta) {
   if (e.scale == nullptr) return;
-  const float r = e.scale[2 * z];
+  const float r = e.scale[z];
   for (int i = 0; i < e.r_power; ++i) alpha *= r;
-  if (e.scale_c) {
-    beta *= r;
-    c_exp = (int)e.scale[2 * z + 1];
-  }
+  if (e.scale_c) beta *= r;
 }
 
 // Two accumulators of neighbouring blocks, 16 rows apart, exchanged between neighbouring groups of
@@ -261,7 +257,7 @@ __device__ __forceinline__ void take(int j, const f4_t (&acc)[S::TM][S::TN],
 // are made once per block column.
 template <class T, class S, bool SLOPE>
 __device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float alpha, float beta,
-                                              int c_exp, int m0, int n0, long z, float* sums_out,
+                                              int m0, int n0, long z, float* sums_out,
                                               const f4_t (&acc)[S::TM][S::TN]) {
   constexpr int NP = S::TM / 2;
   const int row = m0 + 16 * ((lane >> 4) & 1) + 8 * (lane >> 5), col = n0 + (lane & 15);
@@ -323,13 +319,15 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float
             load8(RTAT_TYPE_F32, in, in_at + 32 * q, c);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              v[q][i] = __builtin_fmaf(beta, __builtin_ldexpf(c[i], c_exp), v[q][i]);
+              v[q][i] = __builtin_fmaf(beta, c[i], v[q][i]);
           }
-        } else if (in_type == Half<T>::id) {
-          add_scaled<NP>(Half<T>::id, now, beta, c_exp, v);
-        } else {  // an f16 product that adds to bf16
-          add_scaled<NP>(RTAT_TYPE_BF16, now, beta, c_exp, v);
+        } else {
+          add_scaled<NP>(Half<T>::id, now, beta, v);
         }
+      }
+      if (e.diag != 0.0f) {
+#pragma unroll
+        for (int q = 0; q < NP; ++q) add_diagonal(e.diag, row + 32 * q, col + 16 * j, v[q]);
       }
     }
     in_at += 16 * ldin;
@@ -380,23 +378,21 @@ __device__ __forceinline__ void finish_tile(const Gemm16Args& p, unsigned char* 
   const int m0 = tile_m * S::BM + (wave % S::WGM) * S::WTM;  // of the wave tile
   const int n0 = tile_n * S::BN + (wave / S::WGM) * S::WTN;
   float alpha = e.alpha, beta = e.beta;
-  int c_exp = 0;
-  scale_factors(e, z, alpha, beta, c_exp);
+  scale_factors(e, z, alpha, beta);
   // One row of partial sums per wave column.
   float* sums_out =
       e.sums != nullptr ? e.sums + (long)(tile_n * S::WGN + wave / S::WGM) * e.rows : nullptr;
   // The slices of a triangular product are mirrored when they are joined.
   const bool mirror = p.tri != 0 && tile_m != tile_n && p.slices == 1;
-  const bool inside = m0 + S::WTM <= e.rows && n0 + S::WTN <= e.cols &&
-                      (e.C == nullptr || (m0 + S::WTM <= e.c_rows && n0 + S::WTN <= e.c_cols));
+  const bool inside = m0 + S::WTM <= e.rows && n0 + S::WTN <= e.cols;
   if (inside) {
     if (e.plain)
       finish_plain<T, S>(alpha,
                          static_cast<uint16_t*>(e.D) + z * e.d_stride + m0 +
                              16 * ((lane >> 4) & 1) + 8 * (lane >> 5) + (n0 + (lane & 15)) * e.ldd,
                          e.ldd, acc);
-    else if (e.slope) finish_inside<T, S, true>(e, lane, alpha, beta, c_exp, m0, n0, z, sums_out, acc);
-    else finish_inside<T, S, false>(e, lane, alpha, beta, c_exp, m0, n0, z, sums_out, acc);
+    else if (e.slope) finish_inside<T, S, true>(e, lane, alpha, beta, m0, n0, z, sums_out, acc);
+    else finish_inside<T, S, false>(e, lane, alpha, beta, m0, n0, z, sums_out, acc);
     if (!mirror) return;
   }
   const Parked<S> k(lds, wave, lane);
@@ -411,7 +407,7 @@ __device__ __forceinline__ void finish_tile(const Gemm16Args& p, unsigned char* 
       for (int q = 0; q < Parked<S>::PASSES; ++q) {
         float v[8];
         k.get(q, v);
-        epilogue8(e, alpha, beta, c_exp, m0 + k.row, n0 + 16 * j + q * Parked<S>::CPP + k.col, z, v);
+        epilogue8(e, alpha, beta, m0 + k.row, n0 + 16 * j + q * Parked<S>::CPP + k.col, z, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) sums[i] += v[i];
       }
@@ -421,7 +417,7 @@ __device__ __forceinline__ void finish_tile(const Gemm16Args& p, unsigned char* 
       for (int r0 = 0; r0 < S::WTM; r0 += 32) {
         float v[8];
         k.get_mirrored(r0, v);
-        epilogue8(e, alpha, beta, c_exp, n0 + 16 * j + 8 * (lane & 1), m0 + r0 + (lane >> 1), z, v);
+        epilogue8(e, alpha, beta, n0 + 16 * j + 8 * (lane & 1), m0 + r0 + (lane >> 1), z, v);
       }
     }
   }
@@ -756,21 +752,20 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs p) {
     }
   }
   float alpha = e.alpha, beta = e.beta;
-  int c_exp = 0;
-  scale_factors(e, 0, alpha, beta, c_exp);
+  scale_factors(e, 0, alpha, beta);
   const bool mirror = p.tri != 0 && blockIdx.x != blockIdx.y * JOIN_COLS / JOIN_ROWS;
   if (mirror || e.sums != nullptr) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) part[lc][lr + i] = v[i];
   }
-  epilogue8(e, alpha, beta, c_exp, row, col, 0, v);
+  epilogue8(e, alpha, beta, row, col, 0, v);
   if (mirror) {
     // The same values as sixteen rows of the mirrored columns.
     __syncthreads();
     const int r = t >> 1, c = 8 * (t & 1);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = part[c + i][r];
-    epilogue8(e, alpha, beta, c_exp, blockIdx.y * JOIN_COLS + c, blockIdx.x * JOIN_ROWS + r, 0, v);
+    epilogue8(e, alpha, beta, blockIdx.y * JOIN_COLS + c, blockIdx.x * JOIN_ROWS + r, 0, v);
   }
   if (e.sums == nullptr) return;  // only gradients have them, and those are never triangular
 #pragma unroll
@@ -814,8 +809,8 @@ rtat_status_t launch_kernel(rtat_native_handle* h, const Gemm16& g, Gemm16Args p
   j.slices = p.slices;
   j.tri = p.tri;
   Epilogue raw = {};
-  raw.rows = raw.c_rows = p.m;
-  raw.cols = raw.c_cols = p.n;
+  raw.rows = p.m;
+  raw.cols = p.n;
   raw.alpha = 1.0f;
   raw.D = h->split_ws;
   raw.ldd = j.ldp;
@@ -943,7 +938,7 @@ rtat_status_t launch_gemm16(rtat_native_handle* h, const Gemm16& g) {
   p.ep = g.ep;
   const Epilogue& e = g.ep;
   p.ep.plain = !e.slope && e.act == RTAT_ACT_NONE && e.bias == nullptr && e.aux == nullptr &&
-               e.C == nullptr && e.copy == nullptr && e.d_type == g.type;
+               e.C == nullptr && e.copy == nullptr && e.diag == 0.0f && e.d_type == g.type;
   return g.type == RTAT_TYPE_BF16 ? launch_type<__bf16>(h, g, p) : launch_type<_Float16>(h, g, p);
 }
 
