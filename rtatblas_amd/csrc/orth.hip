@@ -85,14 +85,10 @@ __global__ __launch_bounds__(256) void norm_kernel(NormArgs p) {
   if (threadIdx.x == 0) p.parts[z * p.blocks + blockIdx.x] = s;
 }
 
-// The power of two 2^e at or below X_SCALE / norm, and the ratio r that is left.  The ratio is NaN,
-// and through it every element of the result, for a G that holds an infinity or a NaN (the quotient
-// is 0 or NaN) and for a zero norm without eps (infinite).
-__device__ inline int norm_exponent(const NormArgs& p, long z, double* lds, double& r) {
-  double s = 0.0;
-  for (int i = threadIdx.x; i < p.blocks; i += 256) s += p.parts[z * p.blocks + i];
-  s = block_sum(s, lds);
-  const double want = (double)X_SCALE / (sqrt(s) + (double)p.eps);
+// The power of two 2^e at or below `want` = X_SCALE / norm, and the ratio r that is left.  The ratio
+// is NaN, and through it every element of the result, for a G that holds an infinity or a NaN (the
+// quotient is 0 or NaN) and for a zero norm without eps (infinite).
+__device__ inline int exponent_of(double want, double& r) {
   if (!(want > 0.0) || want - want != 0.0) {
     r = __builtin_nan("");
     return 0;
@@ -100,6 +96,12 @@ __device__ inline int norm_exponent(const NormArgs& p, long z, double* lds, doub
   const int e = ilogb(want);
   r = ldexp(want, -e);
   return e;
+}
+__device__ inline int norm_exponent(const NormArgs& p, long z, double* lds, double& r) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < p.blocks; i += 256) s += p.parts[z * p.blocks + i];
+  s = block_sum(s, lds);
+  return exponent_of((double)X_SCALE / (sqrt(s) + (double)p.eps), r);
 }
 
 __device__ inline void put_x(const NormArgs& p, long z, int row, int col, int e, float (&v)[8]) {
@@ -170,6 +172,225 @@ __global__ __launch_bounds__(256) void turn_kernel(NormArgs p) {
   }
 }
 
+// ---- sides of at most 128: the whole iteration in one workgroup --------------------------------
+//
+// At these sizes the products take less time than the launches between them (128 x 128, five
+// steps: 17 launches 95 us), so a workgroup keeps a matrix to itself: X, M and P in LDS as SIDE
+// rows of SIDE f16, X besides in registers in f32, where the four waves' accumulators lie anyway
+// (wave tiles of SIDE / 2 squared, the same place in every product).  M and P are whole: the
+// half that symmetry would save is not worth the extra steps.
+//
+// LDS rows are the short side of X, so X^T X reads both operands as they lie and X P reads X
+// transposing.  Chunk c of row r lies at c ^ key(r): eight rows that are read together, or the
+// eight rows of a transposing read, fall on different banks.
+struct SmallArgs {
+  NormArgs g;  // G; no scratch
+  int turn;    // 1: X is G^T
+  int steps;
+  uint16_t* O;
+  long ldo, stride_o;
+  float coeffs[3 * RTAT_NEWTON_SCHULZ_MAX_STEPS];
+};
+
+template <int SIDE>
+struct Square {
+  static constexpr int ROW = SIDE * 2, BYTES = SIDE * ROW, T = SIDE / 32;  // T: blocks per wave side
+  __device__ static inline int key(int r) {
+    if (SIDE == 128) return 2 * ((r & 3) | ((r >> 1) & 4)) | ((r >> 2) & 1);
+    return 2 * (((r >> 1) & 1) | ((r >> 2) & 2)) | ((r >> 2) & 1);
+  }
+  // Byte of element k (a multiple of 4) of row r.
+  __device__ static inline int at(int r, int k) {
+    return r * ROW + (((k >> 3) ^ key(r)) * 16) + (k & 4) * 2;
+  }
+  // MFMA operand: sixteen rows from `row` on, K-step `step`.
+  __device__ static inline s8_t rows(const unsigned char* x, int row, int step, int lane) {
+    return *reinterpret_cast<const s8_t*>(x + at(row + (lane & 15), 32 * step + 8 * (lane >> 4)));
+  }
+  // ... sixteen columns from `col` on: k runs down the rows.
+  __device__ static inline s8_t cols(const unsigned char* x, int col, int step, int lane) {
+    typedef __attribute__((address_space(3))) s4_t* lds4_t;
+    const int k = 32 * step + 8 * (lane >> 4) + ((lane & 15) >> 2), c = col + 4 * (lane & 3);
+    const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(x + at(k, c)));
+    const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(x + at(k + 4, c)));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  // acc = (rows or columns of A) times (rows of B) for the wave tile at (m0, n0).
+  template <bool COLS>
+  __device__ static inline void multiply(const unsigned char* A, const unsigned char* B, int m0,
+                                         int n0, int lane, f4_t (&acc)[T][T]) {
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+      for (int j = 0; j < T; ++j) acc[i][j] = f4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int step = 0; step < SIDE / 32; ++step) {
+      s8_t a[T], b[T];
+#pragma unroll
+      for (int i = 0; i < T; ++i)
+        a[i] = COLS ? cols(A, m0 + 16 * i, step, lane) : rows(A, m0 + 16 * i, step, lane);
+#pragma unroll
+      for (int j = 0; j < T; ++j) b[j] = rows(B, n0 + 16 * j, step, lane);
+#pragma unroll
+      for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int j = 0; j < T; ++j) acc[i][j] = Half<_Float16>::mfma(a[i], b[j], acc[i][j]);
+    }
+  }
+  // Four neighbouring elements of row r in f16.
+  __device__ static inline void put(unsigned char* x, int r, int k, const f4_t& v) {
+    typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<h4_t*>(x + at(r, k)) =
+        h4_t{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+  }
+  __device__ static inline f4_t get(const unsigned char* x, int r, int k) {
+    typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+    const h4_t h = *reinterpret_cast<const h4_t*>(x + at(r, k));
+    return f4_t{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+  }
+};
+
+template <int SIDE>
+__global__ __launch_bounds__(256) void small_kernel(SmallArgs p) {
+  typedef Square<SIDE> Q;
+  constexpr int T = Q::T;
+  extern __shared__ __align__(16) unsigned char lds[];
+  __shared__ double sums[4];
+  unsigned char *X = lds, *M = lds + Q::BYTES, *P = lds + 2 * Q::BYTES;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int m0 = (wave & 1) * (SIDE / 2), n0 = (wave >> 1) * (SIDE / 2);
+  const long z = blockIdx.x, g0 = z * p.g.stride_g;
+  // This lane's accumulators: rows (of the long side) hi0 + 16 i .. + 3, columns lo0 + 16 j.
+  const int hi0 = m0 + 4 * (lane >> 4), lo0 = n0 + (lane & 15);
+
+  // G in pieces of eight rows of a column: their squares, then X.
+  constexpr int PIECES = SIDE * SIDE / 8 / 256;
+  float v[PIECES][8];
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int piece = i * 256 + t, row = piece % (SIDE / 8) * 8, col = piece / (SIDE / 8);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[i][q] = 0.0f;
+    if (col < p.g.n && row < p.g.m) rows8(p.g, g0 + (long)col * p.g.ldg, row, v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+    for (int q = 0; q < 8; ++q) s += (double)v[i][q] * (double)v[i][q];
+  s = block_sum(s, sums);
+  double ratio;
+  const int e = exponent_of((double)X_SCALE / (sqrt(s) + (double)p.g.eps), ratio);
+  const float r = (float)ratio;
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int piece = i * 256 + t, row = piece % (SIDE / 8) * 8, col = piece / (SIDE / 8);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[i][q] = __builtin_ldexpf(v[i][q], e);
+    if (!p.turn) {
+      Q::put(X, col, row, f4_t{v[i][0], v[i][1], v[i][2], v[i][3]});
+      Q::put(X, col, row + 4, f4_t{v[i][4], v[i][5], v[i][6], v[i][7]});
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        *reinterpret_cast<_Float16*>(X + Q::at(row + q, col & ~3) + (col & 3) * 2) = (_Float16)v[i][q];
+    }
+  }
+  __syncthreads();
+  f4_t x[T][T];
+#pragma unroll
+  for (int i = 0; i < T; ++i)
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+      const int hi = hi0 + 16 * i, lo = lo0 + 16 * j;
+      if (p.g.type != RTAT_TYPE_F32) {
+        x[i][j] = Q::get(X, lo, hi);  // exact
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int row = p.turn ? lo : hi + q, col = p.turn ? hi + q : lo;
+          const bool in = row < p.g.m && col < p.g.n;
+          const float g = in ? static_cast<const float*>(p.g.G)[g0 + row + (long)col * p.g.ldg] : 0.0f;
+          x[i][j][q] = __builtin_ldexpf(g, e);
+        }
+      }
+    }
+
+  f4_t acc[T][T];
+#pragma unroll 1
+  for (int step = 0; step < p.steps; ++step) {
+    const float ca = p.coeffs[3 * step], cb = p.coeffs[3 * step + 1], cc = p.coeffs[3 * step + 2];
+    const float f = step == 0 ? r : 1.0f;
+    const bool adds = step < p.steps - 2, last = step == p.steps - 1;
+    Q::template multiply<false>(X, X, m0, n0, lane, acc);  // M = X^T X
+    const float am = f * f * (M_SCALE / (X_SCALE * X_SCALE));
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+      for (int j = 0; j < T; ++j) Q::put(M, lo0 + 16 * j, hi0 + 16 * i, acc[i][j] * am);
+    __syncthreads();
+    Q::template multiply<false>(M, M, m0, n0, lane, acc);  // P = b M + c M^2 (+ a)
+    const float ap = cc * (P_SCALE / (M_SCALE * M_SCALE)), bp = cb * (P_SCALE / M_SCALE);
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+      for (int j = 0; j < T; ++j) {
+        const int row = hi0 + 16 * i, col = lo0 + 16 * j;
+        f4_t w = acc[i][j] * ap + Q::get(M, col, row) * bp;
+        if (!adds) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) w[q] += row + q == col ? ca * P_SCALE : 0.0f;
+        }
+        Q::put(P, col, row, w);
+      }
+    __syncthreads();
+    Q::template multiply<true>(X, P, m0, n0, lane, acc);  // X P (+ a X)
+    const float ax = f / P_SCALE, bx = ca * f;
+    __syncthreads();  // X has been read
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+      for (int j = 0; j < T; ++j) {
+        f4_t w = acc[i][j] * ax;
+        if (adds) w += x[i][j] * bx;
+        x[i][j] = w;
+        if (!last) Q::put(X, lo0 + 16 * j, hi0 + 16 * i, w);
+      }
+    __syncthreads();
+  }
+  uint16_t* O = p.O + z * p.stride_o;
+#pragma unroll
+  for (int i = 0; i < T; ++i)
+#pragma unroll
+    for (int j = 0; j < T; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int hi = hi0 + 16 * i + q, lo = lo0 + 16 * j;
+        const int row = p.turn ? lo : hi, col = p.turn ? hi : lo;
+        if (row < p.g.m && col < p.g.n)
+          O[row + (long)col * p.ldo] = float_to_half(RTAT_TYPE_BF16, x[i][j][q] * (1.0f / X_SCALE));
+      }
+}
+
+template <int SIDE>
+rtat_status_t launch_small(rtat_native_handle* h, const SmallArgs& a, int batch) {
+  constexpr int LDS = 3 * Square<SIDE>::BYTES;
+  static PerDeviceOnce configured;
+  if (!configured(h->device, [&] {
+        if (LDS <= 65536) return true;
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(&small_kernel<SIDE>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, LDS) == hipSuccess)
+          return true;
+        (void)hipGetLastError();
+        return false;
+      }))
+    return RTAT_STATUS_NOT_SUPPORTED;
+  hipLaunchKernelGGL((small_kernel<SIDE>), dim3((unsigned)batch), dim3(256), LDS, h->stream, a);
+  return launch_status();
+}
+
+bool is_small(int m, int n) { return m <= 128 && n <= 128; }
+
 struct Layout {
   long hp, lp;                                 // padded sides, the longer first
   size_t x, p;                                 // elements of X and of M
@@ -225,7 +446,7 @@ Gemm16 step_product(int batch, int m, int n, int k, bool ta, bool tb, const void
 }  // namespace
 
 size_t newton_schulz_workspace_bytes(int m, int n, int batch) {
-  if (m <= 0 || n <= 0 || batch <= 0) return 0;
+  if (m <= 0 || n <= 0 || batch <= 0 || is_small(m, n)) return 0;
   return layout_of(m, n, batch).total + 256;
 }
 
@@ -233,6 +454,25 @@ rtat_status_t launch_newton_schulz(rtat_native_handle* h, int g_type, int m, int
                                    const void* G, long ldg, long stride_g, int steps,
                                    const float* coeffs, float eps, void* O, long ldo,
                                    long stride_o) {
+  NormArgs a = {};
+  a.type = g_type;
+  a.m = m;
+  a.n = n;
+  a.G = G;
+  a.ldg = ldg;
+  a.stride_g = stride_g;
+  a.eps = eps;
+  if (is_small(m, n)) {
+    SmallArgs q = {};
+    q.g = a;
+    q.turn = m < n;
+    q.steps = steps;
+    q.O = static_cast<uint16_t*>(O);
+    q.ldo = ldo;
+    q.stride_o = stride_o;
+    for (int i = 0; i < 3 * steps; ++i) q.coeffs[i] = coeffs[i];
+    return m <= 64 && n <= 64 ? launch_small<64>(h, q, batch) : launch_small<128>(h, q, batch);
+  }
   const Layout l = layout_of(m, n, batch);
   unsigned char* ws =
       static_cast<unsigned char*>(acquire_workspace(h, newton_schulz_workspace_bytes(m, n, batch)));
@@ -249,19 +489,11 @@ rtat_status_t launch_newton_schulz(rtat_native_handle* h, int g_type, int m, int
   // Whether step i adds a X rather than putting a on the polynomial's diagonal.
   auto adds = [&](int i) { return i < steps - 2; };
 
-  NormArgs a = {};
-  a.type = g_type;
-  a.m = m;
-  a.n = n;
   auto blocks_for = [](long pieces) {  // two pieces a thread
     const long b = (pieces + 511) / 512;
     return (int)(b < NORM_BLOCKS ? b : NORM_BLOCKS);
   };
   a.blocks = blocks_for((((long)m + 7) / 8) * n);
-  a.G = G;
-  a.ldg = ldg;
-  a.stride_g = stride_g;
-  a.eps = eps;
   a.parts = reinterpret_cast<double*>(ws + l.parts);
   a.scale = scale;
   a.xr = hp;
