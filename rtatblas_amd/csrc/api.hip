@@ -582,6 +582,7 @@ rtat_status_t rtat_gemm_dact(rtat_handle_t h, rtat_type_t type, rtat_operation_t
   if (dbias == nullptr) return launch_gemm16(h, g);
   g.ep.sums = static_cast<float*>(acquire_workspace(h, dbias_workspace_bytes(m, n)));
   if (g.ep.sums == nullptr) return RTAT_STATUS_ALLOC_FAILED;
+  g.scratch_used = dbias_workspace_bytes(m, n);
   st = launch_gemm16(h, g);
   if (st != RTAT_STATUS_SUCCESS) return st;
   return launch_sum_rows(h, g.ep.sums, h->sum_rows, m, dbias);

@@ -16,6 +16,10 @@ struct Gemm16 {
   long lda, a_stride;
   const void* B;
   long ldb, b_stride;
+  // 1: memory behind the operand's last column may be read up to a multiple of 8 rows.
+  int a_roomy, b_roomy;
+  // Bytes at the front of the handle's scratch that the caller uses for this product.
+  size_t scratch_used;
   Epilogue ep;
 };
 

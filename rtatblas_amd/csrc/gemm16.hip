@@ -35,6 +35,9 @@ struct Gemm16Args {
   long lda, a_stride;
   const uint16_t* B;
   long ldb, b_stride;
+  // 1: memory behind the last column of a column-wise operand may be read up to a multiple of 8
+  // rows, so that a panel with that column needs no guards.
+  int a_roomy, b_roomy;
   Epilogue ep;
 };
 
@@ -619,7 +622,8 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
   const int panels = (k_len + BK16 - 1) / BK16;
   const bool ragged = k_len % BK16 != 0 ||
                       (k_first + k_len == p.k &&
-                       ((!KA && m0 + S::BM > p.m) || (!KB && n0 + S::BN > p.n)));
+                       ((!KA && !p.a_roomy && m0 + S::BM > p.m) ||
+                        (!KB && !p.b_roomy && n0 + S::BN > p.n)));
   const int whole = panels - (ragged ? 1 : 0);
   // Item 2 kt is A of panel kt, item 2 kt + 1 its B; item x lies in slot x % 5.
   static_assert(S::BM == S::BN && S::LDS >= 5 * PA::BYTES, "slots of one size");
@@ -878,6 +882,96 @@ int slices_for(const rtat_native_handle* h, const Gemm16& g, long tiles, long sl
   return best;
 }
 
+// Operands that may not go straight to LDS, laid out anew: columns of `rows` elements, `ldd` apart
+// (a multiple of 8) with zeros behind them, and zero columns up to `cols_out`.
+struct PackJob {
+  const uint16_t* src;
+  long ld;
+  int rows, cols, cols_out;
+  uint16_t* dst;
+  long ldd;
+};
+struct PackArgs {
+  PackJob job[2];
+};
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
+  const PackJob j = p.job[blockIdx.y];
+  const int per_col = (int)(j.ldd / 8);
+  const long pieces = (long)per_col * j.cols_out, step = 256L * gridDim.x;
+#pragma unroll 4
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < pieces; i += step) {
+    const int col = (int)(i / per_col), row = (int)(i - (long)col * per_col) * 8;
+    const uint16_t* at = j.src + (long)col * j.ld + row;
+    s8_t v = {};
+    if (col < j.cols && row + 8 <= j.rows) {
+      v = __builtin_bit_cast(s8_t, load16(at, 0));
+    } else if (col < j.cols) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = row + e < j.rows ? (short)at[e] : (short)0;
+    }
+    *reinterpret_cast<s8_t*>(j.dst + (long)col * j.ldd + row) = v;
+  }
+}
+
+// Copies the operands of a product that are not aligned into scratch, if that pays and the scratch
+// is there; true if both operands are direct afterwards.  Worth it when what the faster kernel
+// saves (200 against 700 flop per ps where both were measured, around 2 to 13 GFLOP) is more than
+// a launch and one trip of the operands through memory.
+constexpr size_t PACK_MOST = (size_t)512 << 20;
+bool pack_operands(rtat_native_handle* h, const Gemm16& g, Gemm16Args& p, bool direct_a,
+                   bool direct_b) {
+  if (g.batch != 1 || p.k == 0) return false;
+  const bool both = !direct_a && !direct_b;
+  const int k_out = both ? (p.k + BK16 - 1) / BK16 * BK16 : p.k;
+  auto plan = [&](bool kmajor, const uint16_t* src, long ld, int mn) {
+    PackJob j = {};
+    j.src = src;
+    j.ld = ld;
+    j.rows = kmajor ? p.k : mn;
+    j.cols = kmajor ? mn : p.k;
+    j.cols_out = kmajor ? mn : k_out;
+    j.ldd = ((kmajor ? k_out : mn) + 7L) / 8 * 8;
+    return j;
+  };
+  PackJob a = plan(g.ta, p.A, p.lda, p.m), b = plan(!g.tb, p.B, p.ldb, p.n);
+  const size_t a_bytes = direct_a ? 0 : ((size_t)a.ldd * a.cols_out * 2 + 255) & ~(size_t)255;
+  const size_t b_bytes = direct_b ? 0 : (size_t)b.ldd * b.cols_out * 2;
+  const double gflop = 2e-9 * p.m * (double)p.n * p.k;
+  if (gflop * (1e3 / 200 - 1e3 / 700) < 5.0 + (double)(a_bytes + b_bytes) * 2 / 4e6) return false;
+  const size_t need = g.scratch_used + a_bytes + b_bytes + 256;
+  if (need > PACK_MOST) return false;
+  uint8_t* ws = static_cast<uint8_t*>(acquire_workspace(h, need));
+  if (ws == nullptr) return false;
+  ws = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(ws + g.scratch_used) + 255) & ~(uintptr_t)255);
+  PackArgs q = {};
+  int jobs = 0;
+  long pieces = 0;
+  auto add = [&](PackJob& j, uint8_t* to) {
+    j.dst = reinterpret_cast<uint16_t*>(to);
+    q.job[jobs++] = j;
+    const long n = j.ldd / 8 * j.cols_out;
+    pieces = n > pieces ? n : pieces;
+  };
+  if (!direct_a) {
+    add(a, ws);
+    p.A = a.dst;
+    p.lda = a.ldd;
+    p.a_roomy = 1;
+  }
+  if (!direct_b) {
+    add(b, ws + a_bytes);
+    p.B = b.dst;
+    p.ldb = b.ldd;
+    p.b_roomy = 1;
+  }
+  if (both) p.k = k_out;
+  const long wgs = (pieces + 1023) / 1024;
+  hipLaunchKernelGGL(pack_kernel, dim3((unsigned)(wgs < 4096 ? wgs : 4096), (unsigned)jobs),
+                     dim3(256), 0, h->stream, q);
+  return launch_status() == RTAT_STATUS_SUCCESS;
+}
+
 template <class T>
 rtat_status_t launch_type(rtat_native_handle* h, const Gemm16& g, Gemm16Args p) {
   const long cus = h->compute_units > 0 ? h->compute_units : 256;
@@ -885,7 +979,8 @@ rtat_status_t launch_type(rtat_native_handle* h, const Gemm16& g, Gemm16Args p) 
     const long tm = (p.m + b - 1) / b, tn = (p.n + b - 1) / b;
     return (p.tri ? tm * (tm + 1) / 2 : tm * tn) * g.batch;
   };
-  const bool ring = direct(p.A, p.lda, p.a_stride) && direct(p.B, p.ldb, p.b_stride);
+  const bool direct_a = direct(p.A, p.lda, p.a_stride), direct_b = direct(p.B, p.ldb, p.b_stride);
+  const bool ring = (direct_a && direct_b) || pack_operands(h, g, p, direct_a, direct_b);
   if (ring && tiles(256) >= cus / 2) return launch_ops16<T, S256x256, true>(h, g, p);
   bool large = tiles(128) >= cus;
   double us;
@@ -935,6 +1030,8 @@ rtat_status_t launch_gemm16(rtat_native_handle* h, const Gemm16& g) {
   p.B = static_cast<const uint16_t*>(g.B);
   p.ldb = g.ldb;
   p.b_stride = g.b_stride;
+  p.a_roomy = g.a_roomy;
+  p.b_roomy = g.b_roomy;
   p.ep = g.ep;
   const Epilogue& e = g.ep;
   p.ep.plain = !e.slope && e.act == RTAT_ACT_NONE && e.bias == nullptr && e.aux == nullptr &&

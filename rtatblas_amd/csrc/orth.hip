@@ -435,6 +435,7 @@ Gemm16 step_product(int batch, int m, int n, int k, bool ta, bool tb, const void
   g.B = B;
   g.ldb = ldb;
   g.b_stride = b_stride;
+  g.a_roomy = g.b_roomy = 1;  // padded sides
   g.ep.alpha = alpha;
   g.ep.D = D;
   g.ep.ldd = ldd;
