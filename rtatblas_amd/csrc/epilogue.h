@@ -204,19 +204,58 @@ __device__ inline void store8(int type, void* p, long i, const float (&v)[8]) {
   }
 }
 
-// N times eight elements, 32 apart, from element i on.
-template <int N>
-__device__ inline void store_all(int type, void* p, long i, const float (&v)[N][8]) {
-  if (type == RTAT_TYPE_BF16) {
+// The first `left` of eight neighbours (all of them from 8 on, none up to 0); the others read as 0
+// and are left alone in memory.
+__device__ inline u4_t load16_part(const void* p, long i, int left) {
+  if (left >= 8) return load16(p, 2 * i);
+  const short* at = static_cast<const short*>(p) + i;
+  s8_t v = {};
 #pragma unroll
-    for (int q = 0; q < N; ++q) store8(RTAT_TYPE_BF16, p, i + 32 * q, v[q]);
-  } else if (type == RTAT_TYPE_F16) {
+  for (int e = 0; e < 7; ++e)
+    if (e < left) v[e] = at[e];
+  return __builtin_bit_cast(u4_t, v);
+}
+__device__ inline void load8_part(int type, const void* p, long i, int left, float (&v)[8]) {
+  if (left >= 8) {
+    load8(type, p, i, v);
+  } else if (type == RTAT_TYPE_F32) {
 #pragma unroll
-    for (int q = 0; q < N; ++q) store8(RTAT_TYPE_F16, p, i + 32 * q, v[q]);
+    for (int e = 0; e < 8; ++e) v[e] = e < left ? static_cast<const float*>(p)[i + e] : 0.0f;
   } else {
-#pragma unroll
-    for (int q = 0; q < N; ++q) store8(RTAT_TYPE_F32, p, i + 32 * q, v[q]);
+    unpack8(type, load16_part(p, i, left), v);
   }
+}
+__device__ inline void store8_part(int type, void* p, long i, int left, const float (&v)[8]) {
+  if (left >= 8) {
+    store8(type, p, i, v);
+  } else if (type == RTAT_TYPE_F32) {
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (e < left) static_cast<float*>(p)[i + e] = v[e];
+  } else {
+    const s8_t h = __builtin_bit_cast(s8_t, pack8(type, v));
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (e < left) static_cast<short*>(p)[i + e] = h[e];
+  }
+}
+
+// N times eight elements, 32 apart, from element i on; PART: only the first `left` of all.
+template <int N, bool PART>
+__device__ inline void store_all(int type, void* p, long i, int left, const float (&v)[N][8]) {
+#define RTAT_EACH(A)                                                        \
+  _Pragma("unroll") for (int q = 0; q < N; ++q) {                           \
+    if (PART) store8_part(A, p, i + 32 * q, left - 32 * q, v[q]);           \
+    else store8(A, p, i + 32 * q, v[q]);                                    \
+  }
+  if (type == RTAT_TYPE_BF16) {
+    RTAT_EACH(RTAT_TYPE_BF16)
+  } else if (type == RTAT_TYPE_F16) {
+    RTAT_EACH(RTAT_TYPE_F16)
+  } else {
+    RTAT_EACH(RTAT_TYPE_F32)
+  }
+#undef RTAT_EACH
 }
 
 // N times eight elements through an activation; the choice is made once for all of them.
@@ -325,60 +364,33 @@ __device__ inline void epilogue8(const Epilogue& e, float alpha, float beta, int
   const long c_at = z * e.c_stride + row + (long)col * e.ldc;
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] *= alpha;
-  if (row + 8 <= e.rows) {
-    if (e.slope) {
-      if (e.act != RTAT_ACT_NONE) {
-        const u4_t z[1] = {load16(e.aux, 2 * aux_at)};
-        act_slopes<1>(e.act, e.aux_type, z, reinterpret_cast<float(&)[1][8]>(v));
-      }
-    } else {
-      float c[8];
-      const bool with_c = e.C != nullptr;
-      if (with_c) load8(e.c_type, e.C, c_at, c);
-      if (e.bias != nullptr) {
-        float w[8];
-        load8(e.bias_type, e.bias, row, w);
+  const int left = e.rows - row;
+  if (e.slope) {
+    if (e.act != RTAT_ACT_NONE) {
+      const u4_t z8[1] = {load16_part(e.aux, aux_at, left)};
+      act_slopes<1>(e.act, e.aux_type, z8, reinterpret_cast<float(&)[1][8]>(v));
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += w[i];
-      }
-      if (e.aux != nullptr) store8(e.aux_type, e.aux, aux_at, v);
-      act_values<1>(e.act, reinterpret_cast<float(&)[1][8]>(v));
-      if (with_c) {
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? v[i] : 0.0f;
+  } else {
+    float w[8];
+    if (e.bias != nullptr) {
+      load8_part(e.bias_type, e.bias, row, left, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(beta, c[i], v[i]);
-      }
+      for (int i = 0; i < 8; ++i) v[i] += w[i];
+    }
+    if (e.aux != nullptr) store8_part(e.aux_type, e.aux, aux_at, left, v);
+    act_values<1>(e.act, reinterpret_cast<float(&)[1][8]>(v));
+    if (e.C != nullptr) {
+      load8_part(e.c_type, e.C, c_at, left, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(beta, w[i], v[i]);
     }
     add_diagonal(e.diag, row, col, v);
-    store8(e.d_type, e.D, d_at, v);
-    if (e.copy != nullptr)
-      store8(RTAT_TYPE_F16, e.copy, z * e.copy_stride + row + (long)col * e.ldcopy, v);
-    return;
   }
-#pragma unroll 1
-  for (int i = 0; i < 8; ++i) {
-    // v is indexed by a constant in every copy of this body: no scratch memory.
-    float x = 0.0f;
-#pragma unroll
-    for (int q = 0; q < 8; ++q) x = q == i ? v[q] : x;
-    if (row + i < e.rows) {
-      if (e.slope) {
-        if (e.act != RTAT_ACT_NONE) x *= act_slope(e.act, load_one(e.aux_type, e.aux, aux_at + i));
-      } else {
-        if (e.bias != nullptr) x += load_one(e.bias_type, e.bias, row + i);
-        if (e.aux != nullptr) store_one(e.aux_type, e.aux, aux_at + i, x);
-        x = act_value(e.act, x);
-        if (e.C != nullptr) x = __builtin_fmaf(beta, load_one(e.c_type, e.C, c_at + i), x);
-        if (row + i == col) x += e.diag;
-      }
-      store_one(e.d_type, e.D, d_at + i, x);
-      if (e.copy != nullptr)
-        store_one(RTAT_TYPE_F16, e.copy, z * e.copy_stride + row + (long)col * e.ldcopy + i, x);
-    } else {
-      x = 0.0f;
-    }
-#pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = q == i ? x : v[q];
-  }
+  store8_part(e.d_type, e.D, d_at, left, v);
+  if (e.copy != nullptr)
+    store8_part(RTAT_TYPE_F16, e.copy, z * e.copy_stride + row + (long)col * e.ldcopy, left, v);
 }
 
 }  // namespace rtat_native

@@ -14,11 +14,12 @@
 //     reading: 16 bytes per lane 3.8 with it, 10.3 without; transposing 2.9 with it, 11.0
 //     without (row strides of 128 and 512 bytes).
 //   * The epilogue turns accumulators into eight neighbouring rows per lane, so that bias,
-//     residual, saved activations and results move in 16-byte accesses: by exchanges between
-//     lanes in a tile that lies inside C, through LDS in one that hangs over its edge.
+//     residual, saved activations and results move in 16-byte accesses, by exchanges between
+//     lanes; the mirrored half of a symmetric product passes through LDS.
 #include <type_traits>
 
 #include "gemm16.h"
+#include "gemm16_plan.h"
 #include "gemm_plan.h"
 
 namespace rtat_native {
@@ -41,7 +42,7 @@ struct Gemm16Args {
   Epilogue ep;
 };
 
-constexpr int BK16 = 64;
+constexpr int BK16 = PANEL16;
 
 template <int BM_, int BN_, int WGM_, int WGN_, int OCC_, bool RING_ = false>
 struct Shape16 {
@@ -156,18 +157,14 @@ struct Mover16 {
 };
 
 // A block column (16 columns of C) of a wave tile on its way through the wave's own part of LDS:
-// parked column by column, taken back as eight neighbouring rows per lane or as the mirror image.
+// parked column by column, taken back as its mirror image.
 template <class S>
 struct Parked {
-  static constexpr int LPC = S::WTM / 8;   // lanes per column
-  static constexpr int CPP = 64 / LPC;     // columns per pass
-  static constexpr int PASSES = 16 / CPP;  // passes per block column
   float* park;
-  int lane, row, col;  // this lane's first row of the wave tile, its column within a pass
+  int lane;
 
   __device__ inline Parked(unsigned char* lds, int wave, int lane_)
-      : park(reinterpret_cast<float*>(lds) + wave * 16 * S::PARK), lane(lane_),
-        row((lane_ % LPC) * 8), col(lane_ / LPC) {}
+      : park(reinterpret_cast<float*>(lds) + wave * 16 * S::PARK), lane(lane_) {}
   // Between a wave's writes and its own reads of what other lanes wrote: LDS keeps the order of a
   // wave's accesses, the compiler has to be told.
   __device__ static inline void turn() {
@@ -190,15 +187,6 @@ struct Parked {
       turn();
     } else if constexpr (J + 1 < S::TN) {
       put<J + 1>(j, acc);
-    }
-  }
-  __device__ inline void get(int pass, float (&v)[8]) const {
-    const f4_t* at = reinterpret_cast<const f4_t*>(park + (pass * CPP + col) * S::PARK + row);
-    const f4_t lo = at[0], hi = at[1];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = lo[i];
-      v[4 + i] = hi[i];
     }
   }
   // The block column as rows of the mirrored tile: lane pairs take its two halves.
@@ -253,17 +241,18 @@ __device__ __forceinline__ void take(int j, const f4_t (&acc)[S::TM][S::TN],
   else take<S, (LO + HI) / 2, HI>(j, acc, v);
 }
 
-// A tile that lies wholly inside C: nothing to check, and what a block column needs from memory
-// (the residual, or the argument of the activation) is asked for one block column ahead.  The
-// accumulators stay in registers: a store instruction covers 64 neighbouring bytes of 16 columns.
-// A wave of the largest tile is alone on its SIMD and waits out every taken branch, so choices
-// are made once per block column.
-template <class T, class S, bool SLOPE>
-__device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float alpha, float beta,
-                                              int m0, int n0, long z, float* sums_out,
-                                              const f4_t (&acc)[S::TM][S::TN]) {
+// What a block column needs from memory (the residual, or the argument of the activation) is asked
+// for one block column ahead.  The accumulators stay in registers: a store instruction covers 64
+// neighbouring bytes of 16 columns.  A wave of the largest tile is alone on its SIMD and waits out
+// every taken branch, so choices are made once per block column.  EDGE: the wave tile hangs over
+// the edge of C, and every access asks how many of its eight rows are inside.
+template <class T, class S, bool SLOPE, bool EDGE>
+__device__ __forceinline__ void finish_wave(const Epilogue& e, int lane, float alpha, float beta,
+                                            int m0, int n0, long z, float* sums_out,
+                                            const f4_t (&acc)[S::TM][S::TN]) {
   constexpr int NP = S::TM / 2;
   const int row = m0 + 16 * ((lane >> 4) & 1) + 8 * (lane >> 5), col = n0 + (lane & 15);
+  const int left = e.rows - row;  // of the rows from this lane's first on
   const void* in = SLOPE ? (e.act != RTAT_ACT_NONE ? e.aux : nullptr) : e.C;
   const int in_type = SLOPE ? e.aux_type : e.c_type;
   const long ldin = SLOPE ? e.ldaux : e.ldc;
@@ -276,21 +265,29 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float
   for (int q = 0; q < NP; ++q) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) each[q][i] = 0.0f;
-    if (!SLOPE && e.bias != nullptr) load8(e.bias_type, e.bias, row + 32 * q, each[q]);
+    if (!SLOPE && e.bias != nullptr) {
+      if (EDGE) load8_part(e.bias_type, e.bias, row + 32 * q, left - 32 * q, each[q]);
+      else load8(e.bias_type, e.bias, row + 32 * q, each[q]);
+    }
   }
   // Sixteen-bit values are asked for ahead; 32-bit ones would take twice the registers.
   const bool ahead = in != nullptr && in_type != RTAT_TYPE_F32;
+  auto ask = [&](long at, int c, int q) {
+    if (!EDGE) return load16(in, 2 * (at + 32 * q));
+    return load16_part(in, at + 32 * q, c < e.cols ? left - 32 * q : 0);
+  };
   u4_t next[NP];
 #pragma unroll
-  for (int q = 0; q < NP; ++q) next[q] = ahead ? load16(in, 2 * (in_at + 32 * q)) : u4_t{};
+  for (int q = 0; q < NP; ++q) next[q] = ahead ? ask(in_at, col, q) : u4_t{};
 #pragma unroll 1
   for (int j = 0; j < S::TN; ++j) {
+    const int here = !EDGE || col + 16 * j < e.cols ? left : 0;
     u4_t now[NP];
 #pragma unroll
     for (int q = 0; q < NP; ++q) now[q] = next[q];
     if (ahead && j + 1 < S::TN) {
 #pragma unroll
-      for (int q = 0; q < NP; ++q) next[q] = load16(in, 2 * (in_at + 16 * ldin + 32 * q));
+      for (int q = 0; q < NP; ++q) next[q] = ask(in_at + 16 * ldin, col + 16 * (j + 1), q);
     }
     float v[NP][8];
     take<S>(j, acc, v);
@@ -307,10 +304,10 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float
 #pragma unroll
       for (int q = 0; q < NP; ++q)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) each[q][i] += v[q][i];
+        for (int i = 0; i < 8; ++i) each[q][i] += !EDGE || here > 0 ? v[q][i] : 0.0f;
     } else {
       if (e.aux != nullptr) {
-        store_all<NP>(Half<T>::id, e.aux, aux_at, v);
+        store_all<NP, EDGE>(Half<T>::id, e.aux, aux_at, here, v);
         aux_at += 16 * e.ldaux;
       }
       if (e.act != RTAT_ACT_NONE) act_values<NP>(e.act, v);
@@ -319,10 +316,10 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float
 #pragma unroll
           for (int q = 0; q < NP; ++q) {
             float c[8];
-            load8(RTAT_TYPE_F32, in, in_at + 32 * q, c);
+            if (EDGE) load8_part(RTAT_TYPE_F32, in, in_at + 32 * q, here - 32 * q, c);
+            else load8(RTAT_TYPE_F32, in, in_at + 32 * q, c);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              v[q][i] = __builtin_fmaf(beta, c[i], v[q][i]);
+            for (int i = 0; i < 8; ++i) v[q][i] = __builtin_fmaf(beta, c[i], v[q][i]);
           }
         } else {
           add_scaled<NP>(Half<T>::id, now, beta, v);
@@ -334,10 +331,10 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float
       }
     }
     in_at += 16 * ldin;
-    store_all<NP>(e.d_type, e.D, d_at, v);
+    store_all<NP, EDGE>(e.d_type, e.D, d_at, here, v);
     d_at += 16 * e.ldd;
     if (!SLOPE && e.copy != nullptr) {
-      store_all<NP>(RTAT_TYPE_F16, e.copy, copy_at, v);
+      store_all<NP, EDGE>(RTAT_TYPE_F16, e.copy, copy_at, here, v);
       copy_at += 16 * e.ldcopy;
     }
   }
@@ -349,12 +346,13 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, int lane, float
       for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int d = 1; d < 16; d *= 2) each[q][i] += __shfl_xor(each[q][i], d);
-      if ((lane & 15) == 0) store8(RTAT_TYPE_F32, sums_out, row + 32 * q, each[q]);
+      if ((lane & 15) == 0) store8_part(RTAT_TYPE_F32, sums_out, row + 32 * q, left - 32 * q, each[q]);
     }
   }
 }
 
-// ... whose epilogue is a factor alone and whose result has the operands' type: straight code.
+// A wave tile inside C whose epilogue is a factor alone and whose result has the operands' type:
+// straight code.
 template <class T, class S, int J = 0>
 __device__ __forceinline__ void finish_plain(float alpha, uint16_t* at, long ldd,
                                              const f4_t (&acc)[S::TM][S::TN]) {
@@ -388,53 +386,29 @@ __device__ __forceinline__ void finish_tile(const Gemm16Args& p, unsigned char* 
   // The slices of a triangular product are mirrored when they are joined.
   const bool mirror = p.tri != 0 && tile_m != tile_n && p.slices == 1;
   const bool inside = m0 + S::WTM <= e.rows && n0 + S::WTN <= e.cols;
-  if (inside) {
-    if (e.plain)
-      finish_plain<T, S>(alpha,
-                         static_cast<uint16_t*>(e.D) + z * e.d_stride + m0 +
-                             16 * ((lane >> 4) & 1) + 8 * (lane >> 5) + (n0 + (lane & 15)) * e.ldd,
-                         e.ldd, acc);
-    else if (e.slope) finish_inside<T, S, true>(e, lane, alpha, beta, m0, n0, z, sums_out, acc);
-    else finish_inside<T, S, false>(e, lane, alpha, beta, m0, n0, z, sums_out, acc);
-    if (!mirror) return;
-  }
+  if (inside && e.plain)
+    finish_plain<T, S>(alpha,
+                       static_cast<uint16_t*>(e.D) + z * e.d_stride + m0 +
+                           16 * ((lane >> 4) & 1) + 8 * (lane >> 5) + (n0 + (lane & 15)) * e.ldd,
+                       e.ldd, acc);
+  else if (inside && e.slope)
+    finish_wave<T, S, true, false>(e, lane, alpha, beta, m0, n0, z, sums_out, acc);
+  else if (inside)
+    finish_wave<T, S, false, false>(e, lane, alpha, beta, m0, n0, z, sums_out, acc);
+  else if (e.slope)
+    finish_wave<T, S, true, true>(e, lane, alpha, beta, m0, n0, z, sums_out, acc);
+  else
+    finish_wave<T, S, false, true>(e, lane, alpha, beta, m0, n0, z, sums_out, acc);
+  if (!mirror) return;
   const Parked<S> k(lds, wave, lane);
-  float sums[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) sums[i] = 0.0f;
 #pragma unroll 1
   for (int j = 0; j < S::TN; ++j) {
     k.put(j, acc);
-    if (!inside) {
 #pragma unroll 1
-      for (int q = 0; q < Parked<S>::PASSES; ++q) {
-        float v[8];
-        k.get(q, v);
-        epilogue8(e, alpha, beta, m0 + k.row, n0 + 16 * j + q * Parked<S>::CPP + k.col, z, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sums[i] += v[i];
-      }
-    }
-    if (mirror) {
-#pragma unroll 1
-      for (int r0 = 0; r0 < S::WTM; r0 += 32) {
-        float v[8];
-        k.get_mirrored(r0, v);
-        epilogue8(e, alpha, beta, n0 + 16 * j + 8 * (lane & 1), m0 + r0 + (lane >> 1), z, v);
-      }
-    }
-  }
-  if (sums_out != nullptr) {
-    // Lanes with the same rows add up in a fixed order.
-    constexpr int LPC = Parked<S>::LPC;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int d = LPC; d < 64; d *= 2) sums[i] += __shfl_xor(sums[i], d);
-    if (lane < LPC) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (m0 + k.row + i < e.rows) sums_out[m0 + k.row + i] = sums[i];
+    for (int r0 = 0; r0 < S::WTM; r0 += 32) {
+      float v[8];
+      k.get_mirrored(r0, v);
+      epilogue8(e, alpha, beta, n0 + 16 * j + 8 * (lane & 1), m0 + r0 + (lane >> 1), z, v);
     }
   }
 }
@@ -729,7 +703,6 @@ struct JoinArgs {
   long ldp;
   int slices, tri;
 };
-inline long slice_ld(int m) { return ((long)m + 7) / 8 * 8; }
 
 __global__ __launch_bounds__(256) void join_kernel(JoinArgs p) {
   __shared__ float part[JOIN_COLS][JOIN_ROWS];
@@ -809,7 +782,7 @@ rtat_status_t launch_kernel(rtat_native_handle* h, const Gemm16& g, Gemm16Args p
   JoinArgs j = {};
   j.ep = p.ep;
   j.parts = static_cast<const float*>(h->split_ws);
-  j.ldp = slice_ld(p.m);
+  j.ldp = slice_ld16(p.m);
   j.slices = p.slices;
   j.tri = p.tri;
   Epilogue raw = {};
@@ -855,33 +828,6 @@ bool direct(const void* base, long ld, long stride) {
          ld < (1L << 23);
 }
 
-// Slices for `tiles` tiles on `slots` workgroup slots, at most as many as fill the slots once, each
-// of at least MIN_SLICE panels, that fit the handle's slice scratch: the number with the shortest
-// estimate.  `panel_us`: what a panel of a lone tile takes; the second launch takes 5 us, slices
-// are written and read once at 3 MB/us.  (512 x 512 x 8192 46 -> 19 us, 8192 x 1 x 2048 14 -> 11 us;
-// 1024^3, left whole, takes 7.7 us and would take 16.9 in two.)
-constexpr int MIN_SLICE = 4;
-int slices_for(const rtat_native_handle* h, const Gemm16& g, long tiles, long slots,
-               double panel_us, double& shortest) {
-  const long panels = (g.k + BK16 - 1) / BK16;
-  const long each = slice_ld(g.m) * g.n * 4;
-  shortest = panel_us * (double)panels;
-  if (g.batch != 1 || h->user_ws != nullptr || h->split_ws == nullptr) return 1;
-  long most = slots / tiles;
-  if (most > panels / MIN_SLICE) most = panels / MIN_SLICE;
-  if (most > (long)SPLIT_WS_BYTES / each) most = (long)SPLIT_WS_BYTES / each;
-  int best = 1;
-  for (long s = 2; s <= most; ++s) {
-    const double moved = (double)(2 * s * each) * (g.tri ? 0.5 : 1.0);
-    const double us = panel_us * (double)panels / (double)s + 5.0 + moved / 3e6;
-    if (us < shortest) {
-      shortest = us;
-      best = (int)s;
-    }
-  }
-  return best;
-}
-
 // Operands that may not go straight to LDS, laid out anew: columns of `rows` elements, `ldd` apart
 // (a multiple of 8) with zeros behind them, and zero columns up to `cols_out`.
 struct PackJob {
@@ -894,22 +840,26 @@ struct PackJob {
 struct PackArgs {
   PackJob job[2];
 };
+// A workgroup takes PACK_COLS columns, 32 threads to a column's pieces of eight rows.
+constexpr int PACK_COLS = 32;
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
   const PackJob j = p.job[blockIdx.y];
-  const int per_col = (int)(j.ldd / 8);
-  const long pieces = (long)per_col * j.cols_out, step = 256L * gridDim.x;
-#pragma unroll 4
-  for (long i = blockIdx.x * 256L + threadIdx.x; i < pieces; i += step) {
-    const int col = (int)(i / per_col), row = (int)(i - (long)col * per_col) * 8;
-    const uint16_t* at = j.src + (long)col * j.ld + row;
-    s8_t v = {};
-    if (col < j.cols && row + 8 <= j.rows) {
-      v = __builtin_bit_cast(s8_t, load16(at, 0));
-    } else if (col < j.cols) {
+  const int lane = threadIdx.x % 32, first = blockIdx.x * PACK_COLS + threadIdx.x / 32;
+  for (int row = (blockIdx.z * 32 + lane) * 8; row < j.ldd; row += gridDim.z * 256) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = row + e < j.rows ? (short)at[e] : (short)0;
+    for (int c = 0; c < PACK_COLS; c += 8) {
+      const int col = first + c;
+      if (col >= j.cols_out) continue;
+      const uint16_t* at = j.src + (long)col * j.ld + row;
+      s8_t v = {};
+      if (col < j.cols && row + 8 <= j.rows) {
+        v = __builtin_bit_cast(s8_t, load16(at, 0));
+      } else if (col < j.cols) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = row + e < j.rows ? (short)at[e] : (short)0;
+      }
+      *reinterpret_cast<s8_t*>(j.dst + (long)col * j.ldd + row) = v;
     }
-    *reinterpret_cast<s8_t*>(j.dst + (long)col * j.ldd + row) = v;
   }
 }
 
@@ -945,13 +895,11 @@ bool pack_operands(rtat_native_handle* h, const Gemm16& g, Gemm16Args& p, bool d
   ws = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(ws + g.scratch_used) + 255) & ~(uintptr_t)255);
   PackArgs q = {};
-  int jobs = 0;
-  long pieces = 0;
+  int jobs = 0, cols = 0;
   auto add = [&](PackJob& j, uint8_t* to) {
     j.dst = reinterpret_cast<uint16_t*>(to);
     q.job[jobs++] = j;
-    const long n = j.ldd / 8 * j.cols_out;
-    pieces = n > pieces ? n : pieces;
+    cols = j.cols_out > cols ? j.cols_out : cols;
   };
   if (!direct_a) {
     add(a, ws);
@@ -966,33 +914,30 @@ bool pack_operands(rtat_native_handle* h, const Gemm16& g, Gemm16Args& p, bool d
     p.b_roomy = 1;
   }
   if (both) p.k = k_out;
-  const long wgs = (pieces + 1023) / 1024;
-  hipLaunchKernelGGL(pack_kernel, dim3((unsigned)(wgs < 4096 ? wgs : 4096), (unsigned)jobs),
+  const long ldd = a.ldd > b.ldd ? a.ldd : b.ldd;
+  hipLaunchKernelGGL(pack_kernel,
+                     dim3((unsigned)((cols + PACK_COLS - 1) / PACK_COLS), (unsigned)jobs,
+                          (unsigned)(ldd < 256 * 16 ? (ldd + 255) / 256 : 16)),
                      dim3(256), 0, h->stream, q);
   return launch_status() == RTAT_STATUS_SUCCESS;
 }
 
 template <class T>
 rtat_status_t launch_type(rtat_native_handle* h, const Gemm16& g, Gemm16Args p) {
-  const long cus = h->compute_units > 0 ? h->compute_units : 256;
-  auto tiles = [&](int b) {
-    const long tm = (p.m + b - 1) / b, tn = (p.n + b - 1) / b;
-    return (p.tri ? tm * (tm + 1) / 2 : tm * tn) * g.batch;
-  };
   const bool direct_a = direct(p.A, p.lda, p.a_stride), direct_b = direct(p.B, p.ldb, p.b_stride);
   const bool ring = (direct_a && direct_b) || pack_operands(h, g, p, direct_a, direct_b);
-  if (ring && tiles(256) >= cus / 2) return launch_ops16<T, S256x256, true>(h, g, p);
-  bool large = tiles(128) >= cus;
-  double us;
-  if (!large && p.tri != 0) {
-    // A symmetric product's slices are joined in blocks of the 128 x 128 tile.
-    large = tiles(128) * 2 >= cus;
-    if (large) p.slices = slices_for(h, g, tiles(128), 2 * cus, 0.55, us);
-  }
-  if (large)
-    return ring ? launch_ops16<T, R128x128, true>(h, g, p) : launch_ops16<T, S128x128, false>(h, g, p);
-  if (p.tri == 0) p.slices = slices_for(h, g, tiles(64), 2 * cus, 0.3, us);
-  return ring ? launch_ops16<T, R64x64, true>(h, g, p) : launch_ops16<T, S64x64, false>(h, g, p);
+  // A lent workspace means that the library uses no memory of its own: nothing is cut.
+  const size_t scratch = h->user_ws == nullptr && h->split_ws != nullptr ? SPLIT_WS_BYTES : 0;
+  const Plan16 plan = plan16(p.m, p.n, p.k, g.batch, g.tri != 0, ring, scratch,
+                             h->compute_units > 0 ? h->compute_units : 256);
+  p.tri = plan.tri;
+  p.slices = plan.slices;
+  if (!ring)
+    return plan.tile == 128 ? launch_ops16<T, S128x128, false>(h, g, p)
+                            : launch_ops16<T, S64x64, false>(h, g, p);
+  if (plan.tile == 256) return launch_ops16<T, S256x256, true>(h, g, p);
+  return plan.tile == 128 ? launch_ops16<T, R128x128, true>(h, g, p)
+                          : launch_ops16<T, R64x64, true>(h, g, p);
 }
 
 __global__ __launch_bounds__(256) void sum_rows_kernel(const float* parts, int count, int m,
