@@ -393,4 +393,25 @@ __device__ inline void epilogue8(const Epilogue& e, float alpha, float beta, int
     store8_part(RTAT_TYPE_F16, e.copy, z * e.copy_stride + row + (long)col * e.ldcopy, left, v);
 }
 
+// One element; returns what belongs to its row's sum.
+__device__ inline float epilogue1(const Epilogue& e, float alpha, float beta, int row, int col,
+                                  long z, float x) {
+  x *= alpha;
+  if (e.slope) {
+    if (e.act != RTAT_ACT_NONE)
+      x *= act_slope(e.act, load_one(e.aux_type, e.aux, z * e.aux_stride + row + (long)col * e.ldaux));
+  } else {
+    if (e.bias != nullptr) x += load_one(e.bias_type, e.bias, row);
+    if (e.aux != nullptr) store_one(e.aux_type, e.aux, z * e.aux_stride + row + (long)col * e.ldaux, x);
+    x = act_value(e.act, x);
+    if (e.C != nullptr)
+      x = __builtin_fmaf(beta, load_one(e.c_type, e.C, z * e.c_stride + row + (long)col * e.ldc), x);
+    if (row == col) x += e.diag;
+  }
+  store_one(e.d_type, e.D, z * e.d_stride + row + (long)col * e.ldd, x);
+  if (e.copy != nullptr)
+    store_one(RTAT_TYPE_F16, e.copy, z * e.copy_stride + row + (long)col * e.ldcopy, x);
+  return x;
+}
+
 }  // namespace rtat_native

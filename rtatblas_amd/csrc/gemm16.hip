@@ -828,6 +828,109 @@ bool direct(const void* base, long ld, long stride) {
          ld < (1L << 23);
 }
 
+// Few columns (a single token, or a handful decoded together) of a product whose operands are both
+// contiguous along k: the time is that of reading A once.  A workgroup takes sixteen rows, its
+// waves a share of k each, straight from memory into registers, eight K-steps in flight; the
+// waves' sums meet in LDS.  Sixteen waves read deep enough that 128 workgroups keep memory busy,
+// so nothing is cut across workgroups.  Measured (us; 64 x 64 tiles in slices in brackets):
+// 8192 x 1 x 2048 5.9 (10.9), 2048 x 13 x 8192 9.2 (13.2), 8192 x 16 x 8192 22 (35).
+constexpr int FEW_COLS = 16, FEW_DEEP = 8, FEW_WAVES = 16;
+
+template <class T>
+__global__ __launch_bounds__(64 * FEW_WAVES) void few_columns_kernel(Gemm16Args p) {
+  __shared__ float part[FEW_WAVES][16][17];
+  __shared__ float done[16][17];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, waves = blockDim.x >> 6;
+  const int l16 = lane & 15, q = lane >> 4, m0 = blockIdx.x * 16;
+  // Loads take four neighbouring lanes for the 64 bytes of a row (or column), which memory serves
+  // as one; the MFMA wants them sixteen lanes apart, so each operand is handed round the wave.
+  const int lr = lane >> 2, lq = lane & 3, from = (4 * l16 + q) * 4;
+  const int row = m0 + lr < p.m ? m0 + lr : p.m - 1;
+  // Columns that are not there read the first one again: their sums go nowhere.
+  const uint16_t* a = p.A + (long)row * p.lda + 8 * lq;
+  const uint16_t* b = p.B + (long)(lr < p.n ? lr : 0) * p.ldb + 8 * lq;
+  auto hand = [&](s8_t v) {
+    typedef int i4_t __attribute__((ext_vector_type(4)));
+    const i4_t w = __builtin_bit_cast(i4_t, v);
+    i4_t o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __builtin_amdgcn_ds_bpermute(from, w[i]);
+    return __builtin_bit_cast(s8_t, o);
+  };
+  // Whole K-steps of 32 in batches of FEW_DEEP, dealt to the waves in contiguous shares; the steps
+  // behind the last batch go to the waves one by one.
+  const int steps = p.k / 32, batches = steps / FEW_DEEP, share = (batches + waves - 1) / waves;
+  const int first = wave * share, last = first + share < batches ? first + share : batches;
+  f4_t acc = {0, 0, 0, 0};
+  auto fetch = [&](const uint16_t* at, int step) {
+    return *reinterpret_cast<const s8_t*>(at + 32 * (long)step);
+  };
+  s8_t fa[FEW_DEEP], fb[FEW_DEEP];
+  if (first < last) {
+#pragma unroll
+    for (int u = 0; u < FEW_DEEP; ++u) {
+      fa[u] = fetch(a, first * FEW_DEEP + u);
+      fb[u] = fetch(b, first * FEW_DEEP + u);
+    }
+    for (int s = first + 1; s < last; ++s) {
+#pragma unroll
+      for (int u = 0; u < FEW_DEEP; ++u) {
+        acc = Half<T>::mfma(hand(fa[u]), hand(fb[u]), acc);
+        fa[u] = fetch(a, s * FEW_DEEP + u);
+        fb[u] = fetch(b, s * FEW_DEEP + u);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < FEW_DEEP; ++u) acc = Half<T>::mfma(hand(fa[u]), hand(fb[u]), acc);
+  }
+  for (int s = batches * FEW_DEEP + wave; s < steps; s += waves)
+    acc = Half<T>::mfma(hand(fetch(a, s)), hand(fetch(b, s)), acc);
+  if (wave == waves - 1 && p.k % 32 != 0) {  // k is a multiple of 8: a lane's eight are in or out
+    s8_t ra = {}, rb = {};
+    if (32 * steps + 8 * lq < p.k) {
+      ra = fetch(a, steps);
+      rb = fetch(b, steps);
+    }
+    acc = Half<T>::mfma(hand(ra), hand(rb), acc);
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) part[wave][l16][4 * q + r] = acc[r];
+  __syncthreads();
+  const Epilogue& e = p.ep;
+  if (t < 256) {
+    const int r = t & 15, c = t >> 4;
+    float x = 0.0f;
+    if (c < p.n && m0 + r < p.m) {
+      for (int w = 0; w < waves; ++w) x += part[w][c][r];
+      x = epilogue1(e, e.alpha, e.beta, m0 + r, c, 0, x);
+    }
+    done[c][r] = x;
+  }
+  if (e.sums == nullptr) return;
+  __syncthreads();
+  if (t < 16 && m0 + t < p.m) {
+    float x = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) x += done[c][t];
+    e.sums[m0 + t] = x;
+  }
+}
+
+template <class T>
+rtat_status_t launch_few_columns(rtat_native_handle* h, const Gemm16Args& p) {
+  // Sixteen waves a CU, as far as a workgroup of four to sixteen of them and a batch of K-steps for
+  // each allow (8192 x 16 x 8192: eight 22 us, sixteen 30; 1024 x 16 x 1024: four 5.0, eight 5.7).
+  const long wgs = ((long)p.m + 15) / 16, cus = h->compute_units > 0 ? h->compute_units : 256;
+  long waves = 16 * cus / wgs;
+  const long batches = p.k / (32 * FEW_DEEP);
+  if (waves > batches) waves = batches;
+  waves = waves < 4 ? 4 : (waves > FEW_WAVES ? FEW_WAVES : waves);
+  h->sum_rows = 1;
+  hipLaunchKernelGGL(few_columns_kernel<T>, dim3((unsigned)((p.m + 15) / 16)),
+                     dim3((unsigned)(64 * waves)), 0, h->stream, p);
+  return launch_status();
+}
+
 // Operands that may not go straight to LDS, laid out anew: columns of `rows` elements, `ldd` apart
 // (a multiple of 8) with zeros behind them, and zero columns up to `cols_out`.
 struct PackJob {
@@ -925,6 +1028,9 @@ bool pack_operands(rtat_native_handle* h, const Gemm16& g, Gemm16Args& p, bool d
 template <class T>
 rtat_status_t launch_type(rtat_native_handle* h, const Gemm16& g, Gemm16Args p) {
   const bool direct_a = direct(p.A, p.lda, p.a_stride), direct_b = direct(p.B, p.ldb, p.b_stride);
+  if (g.ta && !g.tb && p.n <= FEW_COLS && direct_a && direct_b && p.k % 8 == 0 && p.k > 0 &&
+      g.batch == 1 && g.tri == 0 && g.ep.scale == nullptr)
+    return launch_few_columns<T>(h, p);
   const bool ring = (direct_a && direct_b) || pack_operands(h, g, p, direct_a, direct_b);
   // A lent workspace means that the library uses no memory of its own: nothing is cut.
   const size_t scratch = h->user_ws == nullptr && h->split_ws != nullptr ? SPLIT_WS_BYTES : 0;
@@ -940,14 +1046,21 @@ rtat_status_t launch_type(rtat_native_handle* h, const Gemm16& g, Gemm16Args p) 
                           : launch_ops16<T, R64x64, true>(h, g, p);
 }
 
+// out[row] = sum of `count` rows of partial sums, in a fixed order: four threads to a row, each a
+// quarter of them.
 __global__ __launch_bounds__(256) void sum_rows_kernel(const float* parts, int count, int m,
                                                        float* out) {
-  const int row = blockIdx.x * 256 + threadIdx.x;
-  if (row >= m) return;
+  __shared__ float quarter[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x * 64 + lane;
   float s = 0.0f;
+  if (row < m) {
 #pragma unroll 8
-  for (int i = 0; i < count; ++i) s += parts[(long)i * m + row];
-  out[row] = s;
+    for (int i = wave; i < count; i += 4) s += parts[(long)i * m + row];
+  }
+  quarter[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && row < m)
+    out[row] = (quarter[0][lane] + quarter[1][lane]) + (quarter[2][lane] + quarter[3][lane]);
 }
 
 }  // namespace
@@ -956,7 +1069,7 @@ int dact_sum_rows(int n) { return 4 * ((n + 63) / 64); }
 
 rtat_status_t launch_sum_rows(rtat_native_handle* h, const float* parts, int count, int m,
                               float* out) {
-  hipLaunchKernelGGL(sum_rows_kernel, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, h->stream,
+  hipLaunchKernelGGL(sum_rows_kernel, dim3((unsigned)((m + 63) / 64)), dim3(256), 0, h->stream,
                      parts, count, m, out);
   return launch_status();
 }
