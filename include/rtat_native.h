@@ -263,7 +263,7 @@ rtat_status_t rtat_strsm_ex(rtat_handle_t handle, rtat_side_t side, rtat_fill_t 
                             const float* alpha, const float* A, int lda, float* B, int ldb,
                             int variant);
 
-/* ---- products of a trained linear layer ------------------------------------------------
+/* ---- products of a trained linear layer --------------------------------------------------
  * Matrix products on 16-bit operands (f32 accumulation on the matrix cores) with the layer's
  * elementwise work in the same launch, the gradients of such a product, and the
  * orthogonalisation of an update to its weight.  No counterpart in the reference.
@@ -273,9 +273,13 @@ rtat_status_t rtat_strsm_ex(rtat_handle_t handle, rtat_side_t side, rtat_fill_t 
  * they are: Y^T (out x tokens) = W X^T is transa = T, transb = N, m = out, n = tokens, k = in,
  * with the row strides as leading dimensions.
  *
- * Any m, n, k, leading dimension and element-aligned pointer is accepted; operands whose base
- * and leading dimension are multiples of 16 bytes are read faster.  An output may not overlap
- * an input or another output unless a function says so. */
+ * Any m, n and k up to 2^31 - 1025 (beyond: RTAT_STATUS_NOT_SUPPORTED), any leading dimension and
+ * element-aligned pointer is accepted; operands whose base and leading dimension are multiples of
+ * 16 bytes are read faster.  Others are first laid out anew in the handle's scratch where that
+ * pays and the scratch is there or may grow (rtat_set_workspace), at most 512 MiB of it.  An output
+ * may not overlap an input or another output unless a function says so.  Results do not depend on
+ * timing; two runs of a call on the same operands and workspace give the same bits.  Work is
+ * enqueued on the handle's stream, on the handle's device whichever one is current. */
 
 /* Element types.  Numeric values equal hipDataType. */
 typedef enum { RTAT_TYPE_F32 = 0, RTAT_TYPE_F16 = 2, RTAT_TYPE_BF16 = 14 } rtat_type_t;

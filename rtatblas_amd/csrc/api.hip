@@ -112,12 +112,18 @@ struct OnDevice {
 bool valid_half(int type) { return type == RTAT_TYPE_F16 || type == RTAT_TYPE_BF16; }
 bool valid_act(int act) { return act >= 0 && act < RTAT_ACT_COUNT; }
 bool short_ld(int ld, int rows) { return ld < (rows > 1 ? rows : 1); }
+// Sizes that still fit an int when they are rounded up to whole tiles.
+bool too_long(int m, int n, int k) {
+  constexpr int most = 0x7fffffff - 1024;
+  return m > most || n > most || k > most;
+}
 
 // Shared checks of the 16-bit products: sizes, and the operands when they are read.
 rtat_status_t check_product(int type, int transa, int transb, int m, int n, int k,
                             const float* alpha, const void* A, int lda, const void* B, int ldb) {
   if (!valid_half(type) || !valid_op(transa) || !valid_op(transb)) return RTAT_STATUS_INVALID_ENUM;
   if (m < 0 || n < 0 || k < 0 || alpha == nullptr) return RTAT_STATUS_INVALID_VALUE;
+  if (too_long(m, n, k)) return RTAT_STATUS_NOT_SUPPORTED;
   if (m == 0 || n == 0 || k == 0 || *alpha == 0.0f) return RTAT_STATUS_SUCCESS;
   if (A == nullptr || B == nullptr || short_ld(lda, transa == RTAT_OP_T ? k : m) ||
       short_ld(ldb, transb == RTAT_OP_T ? n : k))
@@ -503,6 +509,7 @@ rtat_status_t rtat_gemm_ep_backward(rtat_handle_t h, rtat_type_t type, rtat_oper
   if (!valid_half(type) || !valid_op(transa) || !valid_op(transb) || !valid_act(act))
     return RTAT_STATUS_INVALID_ENUM;
   if (m < 0 || n < 0 || k < 0 || alpha == nullptr || grads == nullptr) return RTAT_STATUS_INVALID_VALUE;
+  if (too_long(m, n, k)) return RTAT_STATUS_NOT_SUPPORTED;
   const rtat_gemm_grads_t& q = *grads;
   const bool ta = transa == RTAT_OP_T, tb = transb == RTAT_OP_T;
   const bool want_a = q.dA != nullptr && m > 0 && k > 0, want_b = q.dB != nullptr && n > 0 && k > 0;
@@ -580,7 +587,7 @@ rtat_status_t rtat_gemm_dact(rtat_handle_t h, rtat_type_t type, rtat_operation_t
   g.ep.ldd = ldd;
   g.ep.d_type = type;
   if (dbias == nullptr) return launch_gemm16(h, g);
-  g.ep.sums = static_cast<float*>(acquire_workspace(h, dbias_workspace_bytes(m, n)));
+  g.ep.sums = acquire_sums(h, m, n);
   if (g.ep.sums == nullptr) return RTAT_STATUS_ALLOC_FAILED;
   g.scratch_used = dbias_workspace_bytes(m, n);
   st = launch_gemm16(h, g);
@@ -599,6 +606,7 @@ rtat_status_t rtat_newton_schulz(rtat_handle_t h, rtat_type_t g_type, int m, int
   if (m < 0 || n < 0 || batch < 0 || steps < 1 || steps > RTAT_NEWTON_SCHULZ_MAX_STEPS ||
       coeffs == nullptr || !(eps >= 0.0f))
     return RTAT_STATUS_INVALID_VALUE;
+  if (too_long(m, n, 0)) return RTAT_STATUS_NOT_SUPPORTED;
   if (m == 0 || n == 0 || batch == 0) return RTAT_STATUS_SUCCESS;
   if (G == nullptr || O == nullptr || short_ld(ldg, m) || short_ld(ldo, m))
     return RTAT_STATUS_INVALID_VALUE;

@@ -42,5 +42,7 @@ rtat_status_t launch_act_backward(rtat_native_handle* h, int type, int act, int 
                                   const void* dD, long lddd, const void* Z, long ldz, void* dZ,
                                   long lddz, float* dbias);
 size_t dbias_workspace_bytes(int m, int n);
+// The partial row sums' place in the handle's scratch, aligned; null when it cannot be had.
+float* acquire_sums(rtat_native_handle* h, int m, int n);
 
 }  // namespace rtat_native

@@ -56,6 +56,7 @@ inline Plan16 plan16(int m, int n, int k, int batch, bool symmetric, bool large,
       // The slices of a half are joined in blocks of the 128 x 128 tile.
       long most = batch == 1 && (!tri || b == 128) ? panels / SLICE_PANELS16 : 1;
       if (most > 64) most = 64;
+      if (n > 65535 * 16) most = 1;  // the join's grid
       for (long cut = 1; cut <= (most > 1 ? most : 1); ++cut) {
         if (cut > 1 && (double)cut * each > (double)scratch) break;
         double us = price16(b, tiles * cut, (panels + cut - 1) / cut, cus);

@@ -80,7 +80,12 @@ __global__ __launch_bounds__(256) void act_backward_kernel(ActArgs p) {
 
 size_t dbias_workspace_bytes(int m, int n) {
   if (m <= 0 || n <= 0) return 0;
-  return (size_t)dact_sum_rows(n) * (size_t)m * sizeof(float);
+  return (size_t)dact_sum_rows(n) * (size_t)m * sizeof(float) + 256;  // room to align
+}
+
+float* acquire_sums(rtat_native_handle* h, int m, int n) {
+  const uintptr_t ws = reinterpret_cast<uintptr_t>(acquire_workspace(h, dbias_workspace_bytes(m, n)));
+  return reinterpret_cast<float*>((ws + 255) & ~(uintptr_t)255);
 }
 
 rtat_status_t launch_act_backward(rtat_native_handle* h, int type, int act, int m, int n,
@@ -109,7 +114,7 @@ rtat_status_t launch_act_backward(rtat_native_handle* h, int type, int act, int 
   if (dbias != nullptr) {
     p.sums = dbias;
     if (chunks > 1) {
-      p.sums = static_cast<float*>(acquire_workspace(h, (size_t)chunks * m * sizeof(float)));
+      p.sums = acquire_sums(h, m, n);
       if (p.sums == nullptr) return RTAT_STATUS_ALLOC_FAILED;
     }
   }

@@ -9,7 +9,8 @@ from rtatblas_amd import native
 
 BF16, F16, F32 = native.TYPE_BF16, native.TYPE_F16, native.TYPE_F32
 N, T = native.OP_N, native.OP_T
-OK, INVALID, NULL_HANDLE, ENUM = 0, 3, 9, 10
+OK, INVALID, UNSUPPORTED, NULL_HANDLE, ENUM = 0, 3, 7, 9, 10
+LONG = 2 ** 31 - 1000
 P = 4096                       # a pointer that is never followed
 
 
@@ -41,7 +42,8 @@ def ep(h, **kw):
     (dict(act=5), ENUM), (dict(act=-1), ENUM), (dict(m=-1), INVALID), (dict(n=-1), INVALID), (dict(k=-1), INVALID),
     (dict(lda=3), INVALID), (dict(ldb=1), INVALID), (dict(ldd=3), INVALID), (dict(A=None), INVALID), (dict(B=None), INVALID),
     (dict(D=None), INVALID), (dict(ta=T, lda=1), INVALID), (dict(tb=T, ldb=2), INVALID), (dict(beta=1.0), INVALID),
-    (dict(beta=1.0, C=P, ldc=3), INVALID), (dict(aux=P, ldaux=3), INVALID), (dict(m=0, D=None), OK), (dict(n=0, A=None), OK)])
+    (dict(beta=1.0, C=P, ldc=3), INVALID), (dict(aux=P, ldaux=3), INVALID), (dict(m=0, D=None), OK), (dict(n=0, A=None), OK),
+    (dict(k=LONG, ldb=LONG), UNSUPPORTED), (dict(m=LONG, lda=LONG, ldd=LONG), UNSUPPORTED)])
 def test_gemm_ep(bare, change, status):
     assert ep(bare, **change) == status
 
@@ -65,7 +67,7 @@ def test_null_handle_and_null_scalars(bare):
     (dict(dD=None, dbias=P), INVALID), (dict(lddd=3), INVALID), (dict(act=2, aux=None, dZ=P, lddz=4), INVALID),
     (dict(act=2, aux=P, ldaux=3, dZ=P, lddz=4), INVALID), (dict(act=2, aux=P, ldaux=4, dZ=P, lddz=3), INVALID),
     (dict(act=2, aux=P, ldaux=4, dA=P, ldda=4), INVALID), (dict(dA=P, ldda=4, B=None), INVALID),
-    (dict(dB=P, lddb=2, A=None), INVALID), (dict(dB=P, lddb=2, lda=3), INVALID), (dict(), OK), (dict(m=0, n=0, dD=None), OK)])
+    (dict(dB=P, lddb=2, A=None), INVALID), (dict(dB=P, lddb=2, lda=3), INVALID), (dict(), OK), (dict(m=0, n=0, dD=None), OK), (dict(n=LONG), UNSUPPORTED)])
 def test_backward(bare, change, status):
     a = dict(type=BF16, ta=N, tb=N, m=4, n=3, k=2, alpha=1.0, A=P, lda=4, B=P, ldb=2, dD=P, lddd=4, check=False)
     a.update(change)
@@ -85,7 +87,7 @@ def test_dact(bare, change, status):
     (dict(g_type=5), ENUM), (dict(m=-1), INVALID), (dict(batch=-1), INVALID), (dict(coeffs=[]), INVALID),
     (dict(coeffs=[(1, 1, 1)] * 33), INVALID), (dict(eps=-1.0), INVALID), (dict(eps=float("nan")), INVALID), (dict(G=None), INVALID),
     (dict(O=None), INVALID), (dict(ldg=3), INVALID), (dict(ldo=3), INVALID), (dict(batch=65536), INVALID), (dict(m=0, G=None), OK),
-    (dict(n=0), OK), (dict(batch=0), OK)])
+    (dict(n=LONG), UNSUPPORTED), (dict(n=0), OK), (dict(batch=0), OK)])
 def test_newton_schulz(bare, change, status):
     a = dict(g_type=F32, m=4, n=3, G=P, ldg=4, O=P, ldo=4, coeffs=[(1.5, -0.5, 0.0)], check=False)
     a.update(change)
