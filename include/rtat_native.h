@@ -13,10 +13,12 @@
  *   - matrices are device pointers, column-major, leading dimension in elements;
  *   - alpha/beta are HOST pointers and are read before the call returns;
  *   - work is enqueued on the handle's stream only; nothing synchronises, nothing is
- *     printed, nothing throws: the return value is the only error channel.  One compute
- *     call may allocate: an rtat_dtrsm / rtat_strsm that needs more handle-owned scratch
- *     than any call before it on that handle (one hipMalloc, no synchronisation, no
- *     hipFree; see rtat_set_workspace for how to avoid it);
+ *     printed, nothing throws: the return value is the only error channel.  A compute
+ *     call allocates only where it needs more handle-owned scratch than any call before it
+ *     on that handle: rtat_dtrsm / rtat_strsm, rtat_gemm_ep (operands that it lays out
+ *     anew), rtat_gemm_ep_backward and rtat_gemm_dact (the same, and dbias) and
+ *     rtat_newton_schulz (one hipMalloc, no synchronisation, no hipFree; see
+ *     rtat_set_workspace for how to avoid it);
  *   - with beta == 0 the output is never read (it may hold NaN/Inf);
  *   - m, n or k equal to 0 is legal (quick return / pure scaling);
  *   - enum values are those of hipBLAS so plan files and oracle calls interoperate.
@@ -76,7 +78,8 @@ rtat_status_t rtat_get_stream(rtat_handle_t handle, rtat_stream_t* stream);
 
 /* Lend the handle a caller-owned device buffer for TRSM's scratch: the inverted diagonal
  * blocks and the packed off-diagonal blocks of each 512- or 1024-row panel
- * (the role rocBLAS's handle memory plays under hipblasDtrsm).  Pass (NULL, 0) to go back
+ * (the role rocBLAS's handle memory plays under hipblasDtrsm).  The products of a linear
+ * layer and rtat_newton_schulz take theirs from it too.  Pass (NULL, 0) to go back
  * to the handle-owned buffer.  That one grows by hipMalloc when a call needs more than
  * the handle has; a block that is outgrown is kept until rtat_destroy (enqueued work and
  * captured graphs may still name it) and each new block is at least twice the last, so

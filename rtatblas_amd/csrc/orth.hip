@@ -47,13 +47,18 @@ struct NormArgs {
   long x_stride;
 };
 
+// Sum over a workgroup of WAVES waves, the same order in every thread.
+template <int WAVES>
 __device__ inline double block_sum(double s, double* lds) {
 #pragma unroll
   for (int d = 32; d > 0; d /= 2) s += __shfl_xor(s, d);
   const int wave = threadIdx.x / 64;
   if (threadIdx.x % 64 == 0) lds[wave] = s;
   __syncthreads();
-  return lds[0] + lds[1] + lds[2] + lds[3];
+  s = lds[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) s += lds[w];
+  return s;
 }
 
 // Eight rows of a column from `row` on; rows past m read as zero.
@@ -81,7 +86,7 @@ __global__ __launch_bounds__(256) void norm_kernel(NormArgs p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) s += (double)v[e] * (double)v[e];
   }
-  s = block_sum(s, lds);
+  s = block_sum<4>(s, lds);
   if (threadIdx.x == 0) p.parts[z * p.blocks + blockIdx.x] = s;
 }
 
@@ -100,7 +105,7 @@ __device__ inline int exponent_of(double want, double& r) {
 __device__ inline int norm_exponent(const NormArgs& p, long z, double* lds, double& r) {
   double s = 0.0;
   for (int i = threadIdx.x; i < p.blocks; i += 256) s += p.parts[z * p.blocks + i];
-  s = block_sum(s, lds);
+  s = block_sum<4>(s, lds);
   return exponent_of((double)X_SCALE / (sqrt(s) + (double)p.eps), r);
 }
 
@@ -176,13 +181,15 @@ __global__ __launch_bounds__(256) void turn_kernel(NormArgs p) {
 //
 // At these sizes the products take less time than the launches between them (128 x 128, five
 // steps: 17 launches 95 us), so a workgroup keeps a matrix to itself: X, M and P in LDS as SIDE
-// rows of SIDE f16, X besides in registers in f32, where the four waves' accumulators lie anyway
-// (wave tiles of SIDE / 2 squared, the same place in every product).  M and P are whole: the
-// half that symmetry would save is not worth the extra steps.
+// rows of SIDE f16, X besides in registers in f32, where the waves' accumulators lie anyway (eight
+// wave tiles of SIDE / 2 by SIDE / 4, the same place in every product).  M and P are whole: the
+// half that symmetry would save is not worth the extra steps.  128 x 128, five steps: 29 us with
+// eight waves, 34 with four, which have half as many requests for LDS on their way.
 //
 // LDS rows are the short side of X, so X^T X reads both operands as they lie and X P reads X
 // transposing.  Chunk c of row r lies at c ^ key(r): eight rows that are read together, or the
 // eight rows of a transposing read, fall on different banks.
+constexpr int SMALL_THREADS = 512;
 struct SmallArgs {
   NormArgs g;  // G; no scratch
   int turn;    // 1: X is G^T
@@ -194,7 +201,8 @@ struct SmallArgs {
 
 template <int SIDE>
 struct Square {
-  static constexpr int ROW = SIDE * 2, BYTES = SIDE * ROW, T = SIDE / 32;  // T: blocks per wave side
+  static constexpr int ROW = SIDE * 2, BYTES = SIDE * ROW;
+  static constexpr int TM = SIDE / 32, TN = SIDE / 64;  // blocks of a wave tile
   __device__ static inline int key(int r) {
     if (SIDE == 128) return 2 * ((r & 3) | ((r >> 1) & 4)) | ((r >> 2) & 1);
     return 2 * (((r >> 1) & 1) | ((r >> 2) & 2)) | ((r >> 2) & 1);
@@ -218,23 +226,23 @@ struct Square {
   // acc = (rows or columns of A) times (rows of B) for the wave tile at (m0, n0).
   template <bool COLS>
   __device__ static inline void multiply(const unsigned char* A, const unsigned char* B, int m0,
-                                         int n0, int lane, f4_t (&acc)[T][T]) {
+                                         int n0, int lane, f4_t (&acc)[TM][TN]) {
 #pragma unroll
-    for (int i = 0; i < T; ++i)
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int j = 0; j < T; ++j) acc[i][j] = f4_t{0, 0, 0, 0};
+      for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{0, 0, 0, 0};
 #pragma unroll
     for (int step = 0; step < SIDE / 32; ++step) {
-      s8_t a[T], b[T];
+      s8_t a[TM], b[TN];
 #pragma unroll
-      for (int i = 0; i < T; ++i)
+      for (int i = 0; i < TM; ++i)
         a[i] = COLS ? cols(A, m0 + 16 * i, step, lane) : rows(A, m0 + 16 * i, step, lane);
 #pragma unroll
-      for (int j = 0; j < T; ++j) b[j] = rows(B, n0 + 16 * j, step, lane);
+      for (int j = 0; j < TN; ++j) b[j] = rows(B, n0 + 16 * j, step, lane);
 #pragma unroll
-      for (int i = 0; i < T; ++i)
+      for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < T; ++j) acc[i][j] = Half<_Float16>::mfma(a[i], b[j], acc[i][j]);
+        for (int j = 0; j < TN; ++j) acc[i][j] = Half<_Float16>::mfma(a[i], b[j], acc[i][j]);
     }
   }
   // Four neighbouring elements of row r in f16.
@@ -251,25 +259,25 @@ struct Square {
 };
 
 template <int SIDE>
-__global__ __launch_bounds__(256) void small_kernel(SmallArgs p) {
+__global__ __launch_bounds__(SMALL_THREADS) void small_kernel(SmallArgs p) {
   typedef Square<SIDE> Q;
-  constexpr int T = Q::T;
+  constexpr int TM = Q::TM, TN = Q::TN, NT = SMALL_THREADS;
   extern __shared__ __align__(16) unsigned char lds[];
-  __shared__ double sums[4];
+  __shared__ double sums[NT / 64];
   unsigned char *X = lds, *M = lds + Q::BYTES, *P = lds + 2 * Q::BYTES;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int m0 = (wave & 1) * (SIDE / 2), n0 = (wave >> 1) * (SIDE / 2);
+  const int m0 = (wave & 1) * (SIDE / 2), n0 = (wave >> 1) * (SIDE / 4);
   const long z = blockIdx.x, g0 = z * p.g.stride_g;
   // This lane's accumulators: rows (of the long side) hi0 + 16 i .. + 3, columns lo0 + 16 j.
   const int hi0 = m0 + 4 * (lane >> 4), lo0 = n0 + (lane & 15);
 
   // G in pieces of eight rows of a column: their squares, then X.
-  constexpr int PIECES = SIDE * SIDE / 8 / 256;
+  constexpr int PIECES = SIDE * SIDE / 8 / NT;
   float v[PIECES][8];
   double s = 0.0;
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
-    const int piece = i * 256 + t, row = piece % (SIDE / 8) * 8, col = piece / (SIDE / 8);
+    const int piece = i * NT + t, row = piece % (SIDE / 8) * 8, col = piece / (SIDE / 8);
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[i][q] = 0.0f;
     if (col < p.g.n && row < p.g.m) rows8(p.g, g0 + (long)col * p.g.ldg, row, v[i]);
@@ -278,13 +286,13 @@ __global__ __launch_bounds__(256) void small_kernel(SmallArgs p) {
   for (int i = 0; i < PIECES; ++i)
 #pragma unroll
     for (int q = 0; q < 8; ++q) s += (double)v[i][q] * (double)v[i][q];
-  s = block_sum(s, sums);
+  s = block_sum<NT / 64>(s, sums);
   double ratio;
   const int e = exponent_of((double)X_SCALE / (sqrt(s) + (double)p.g.eps), ratio);
   const float r = (float)ratio;
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
-    const int piece = i * 256 + t, row = piece % (SIDE / 8) * 8, col = piece / (SIDE / 8);
+    const int piece = i * NT + t, row = piece % (SIDE / 8) * 8, col = piece / (SIDE / 8);
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[i][q] = __builtin_ldexpf(v[i][q], e);
     if (!p.turn) {
@@ -297,11 +305,11 @@ __global__ __launch_bounds__(256) void small_kernel(SmallArgs p) {
     }
   }
   __syncthreads();
-  f4_t x[T][T];
+  f4_t x[TM][TN];
 #pragma unroll
-  for (int i = 0; i < T; ++i)
+  for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < T; ++j) {
+    for (int j = 0; j < TN; ++j) {
       const int hi = hi0 + 16 * i, lo = lo0 + 16 * j;
       if (p.g.type != RTAT_TYPE_F32) {
         x[i][j] = Q::get(X, lo, hi);  // exact
@@ -316,7 +324,7 @@ __global__ __launch_bounds__(256) void small_kernel(SmallArgs p) {
       }
     }
 
-  f4_t acc[T][T];
+  f4_t acc[TM][TN];
 #pragma unroll 1
   for (int step = 0; step < p.steps; ++step) {
     const float ca = p.coeffs[3 * step], cb = p.coeffs[3 * step + 1], cc = p.coeffs[3 * step + 2];
@@ -325,16 +333,16 @@ __global__ __launch_bounds__(256) void small_kernel(SmallArgs p) {
     Q::template multiply<false>(X, X, m0, n0, lane, acc);  // M = X^T X
     const float am = f * f * (M_SCALE / (X_SCALE * X_SCALE));
 #pragma unroll
-    for (int i = 0; i < T; ++i)
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int j = 0; j < T; ++j) Q::put(M, lo0 + 16 * j, hi0 + 16 * i, acc[i][j] * am);
+      for (int j = 0; j < TN; ++j) Q::put(M, lo0 + 16 * j, hi0 + 16 * i, acc[i][j] * am);
     __syncthreads();
     Q::template multiply<false>(M, M, m0, n0, lane, acc);  // P = b M + c M^2 (+ a)
     const float ap = cc * (P_SCALE / (M_SCALE * M_SCALE)), bp = cb * (P_SCALE / M_SCALE);
 #pragma unroll
-    for (int i = 0; i < T; ++i)
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int j = 0; j < T; ++j) {
+      for (int j = 0; j < TN; ++j) {
         const int row = hi0 + 16 * i, col = lo0 + 16 * j;
         f4_t w = acc[i][j] * ap + Q::get(M, col, row) * bp;
         if (!adds) {
@@ -348,9 +356,9 @@ __global__ __launch_bounds__(256) void small_kernel(SmallArgs p) {
     const float ax = f / P_SCALE, bx = ca * f;
     __syncthreads();  // X has been read
 #pragma unroll
-    for (int i = 0; i < T; ++i)
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int j = 0; j < T; ++j) {
+      for (int j = 0; j < TN; ++j) {
         f4_t w = acc[i][j] * ax;
         if (adds) w += x[i][j] * bx;
         x[i][j] = w;
@@ -360,9 +368,9 @@ __global__ __launch_bounds__(256) void small_kernel(SmallArgs p) {
   }
   uint16_t* O = p.O + z * p.stride_o;
 #pragma unroll
-  for (int i = 0; i < T; ++i)
+  for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < T; ++j)
+    for (int j = 0; j < TN; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int hi = hi0 + 16 * i + q, lo = lo0 + 16 * j;
@@ -385,7 +393,7 @@ rtat_status_t launch_small(rtat_native_handle* h, const SmallArgs& a, int batch)
         return false;
       }))
     return RTAT_STATUS_NOT_SUPPORTED;
-  hipLaunchKernelGGL((small_kernel<SIDE>), dim3((unsigned)batch), dim3(256), LDS, h->stream, a);
+  hipLaunchKernelGGL((small_kernel<SIDE>), dim3((unsigned)batch), dim3(SMALL_THREADS), LDS, h->stream, a);
   return launch_status();
 }
 
