@@ -276,7 +276,7 @@ rtat_status_t rtat_strsm_ex(rtat_handle_t handle, rtat_side_t side, rtat_fill_t 
  * they are: Y^T (out x tokens) = W X^T is transa = T, transb = N, m = out, n = tokens, k = in,
  * with the row strides as leading dimensions.
  *
- * Any m, n and k up to 2^31 - 1025 (beyond: RTAT_STATUS_NOT_SUPPORTED), any leading dimension and
+ * Any m, n and k up to 2^30 - 1024 (beyond: RTAT_STATUS_NOT_SUPPORTED), any leading dimension and
  * element-aligned pointer is accepted; operands whose base and leading dimension are multiples of
  * 16 bytes are read faster.  Others are first laid out anew in the handle's scratch where that
  * pays and the scratch is there or may grow (rtat_set_workspace), at most 512 MiB of it.  An output
@@ -374,13 +374,15 @@ size_t rtat_dbias_workspace_bytes(int m, int n);
  *   X = G / (||G||_F + eps);  for each of `steps` triples (a, b, c) of `coeffs`:
  *   M = X X^T,  X = a X + (b M + c M^2) X;   O = X
  * (for m > n the same with M = X^T X).  coeffs is a host array of 3 * steps floats, read before
- * the call returns; 1 <= steps <= RTAT_NEWTON_SCHULZ_MAX_STEPS.  Between products X and M are
+ * the call returns; 1 <= steps <= RTAT_NEWTON_SCHULZ_MAX_STEPS, batch <= 65535 and eps finite and
+ * not negative (else RTAT_STATUS_INVALID_VALUE).  Between products X and M are
  * held in f16, scaled so that singular values up to 60 of X fit, and X in f32 as well until the
  * last two steps, so O carries about nine bits: that is why it is BF16 whatever g_type is.
  * G_i = G + i * stride_g, O_i = O + i * stride_o (elements; ignored when batch <= 1); O may be G
  * when g_type is BF16 and the leading dimensions and strides agree.  An infinity or a NaN in G_i
  * makes O_i NaN throughout and no other.
- * Takes rtat_newton_schulz_workspace_bytes of the handle's scratch, as rtat_dtrsm does. */
+ * Takes rtat_newton_schulz_workspace_bytes of the handle's scratch, as rtat_dtrsm does (SIZE_MAX,
+ * and RTAT_STATUS_ALLOC_FAILED from the call, where that would pass 2^60). */
 #define RTAT_NEWTON_SCHULZ_MAX_STEPS 32
 rtat_status_t rtat_newton_schulz(rtat_handle_t handle, rtat_type_t g_type, int m, int n,
                                  int batch, const void* G, int ldg, int64_t stride_g, int steps,

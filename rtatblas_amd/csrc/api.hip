@@ -112,9 +112,9 @@ struct OnDevice {
 bool valid_half(int type) { return type == RTAT_TYPE_F16 || type == RTAT_TYPE_BF16; }
 bool valid_act(int act) { return act >= 0 && act < RTAT_ACT_COUNT; }
 bool short_ld(int ld, int rows) { return ld < (rows > 1 ? rows : 1); }
-// Sizes that still fit an int when they are rounded up to whole tiles.
+// A launch holds fewer than 2^32 threads: 2^30 rows in 64 x 64 tiles of 256 are one too many.
 bool too_long(int m, int n, int k) {
-  constexpr int most = 0x7fffffff - 1024;
+  constexpr int most = (1 << 30) - 1024;
   return m > most || n > most || k > most;
 }
 
@@ -604,7 +604,7 @@ rtat_status_t rtat_newton_schulz(rtat_handle_t h, rtat_type_t g_type, int m, int
   RTAT_CHECK_HANDLE(h);
   if (!valid_half(g_type) && g_type != RTAT_TYPE_F32) return RTAT_STATUS_INVALID_ENUM;
   if (m < 0 || n < 0 || batch < 0 || steps < 1 || steps > RTAT_NEWTON_SCHULZ_MAX_STEPS ||
-      coeffs == nullptr || !(eps >= 0.0f))
+      coeffs == nullptr || !(eps >= 0.0f && eps <= 3.402823466e38f))
     return RTAT_STATUS_INVALID_VALUE;
   if (too_long(m, n, 0)) return RTAT_STATUS_NOT_SUPPORTED;
   if (m == 0 || n == 0 || batch == 0) return RTAT_STATUS_SUCCESS;

@@ -835,6 +835,7 @@ bool direct(const void* base, long ld, long stride) {
 // so nothing is cut across workgroups.  Measured (us; 64 x 64 tiles in slices in brackets):
 // 8192 x 1 x 2048 5.9 (10.9), 2048 x 13 x 8192 9.2 (13.2), 8192 x 16 x 8192 22 (35).
 constexpr int FEW_COLS = 16, FEW_DEEP = 8, FEW_WAVES = 16;
+constexpr int FEW_ROWS = 1 << 27;  // 2^23 workgroups of 256: a launch holds fewer than 2^32 threads
 
 template <class T>
 __global__ __launch_bounds__(64 * FEW_WAVES) void few_columns_kernel(Gemm16Args p) {
@@ -997,6 +998,7 @@ bool pack_operands(rtat_native_handle* h, const Gemm16& g, Gemm16Args& p, bool d
   if (ws == nullptr) return false;
   ws = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(ws + g.scratch_used) + 255) & ~(uintptr_t)255);
+  const Gemm16Args before = p;
   PackArgs q = {};
   int jobs = 0, cols = 0;
   auto add = [&](PackJob& j, uint8_t* to) {
@@ -1022,14 +1024,16 @@ bool pack_operands(rtat_native_handle* h, const Gemm16& g, Gemm16Args& p, bool d
                      dim3((unsigned)((cols + PACK_COLS - 1) / PACK_COLS), (unsigned)jobs,
                           (unsigned)(ldd < 256 * 16 ? (ldd + 255) / 256 : 16)),
                      dim3(256), 0, h->stream, q);
-  return launch_status() == RTAT_STATUS_SUCCESS;
+  if (launch_status() == RTAT_STATUS_SUCCESS) return true;
+  p = before;
+  return false;
 }
 
 template <class T>
 rtat_status_t launch_type(rtat_native_handle* h, const Gemm16& g, Gemm16Args p) {
   const bool direct_a = direct(p.A, p.lda, p.a_stride), direct_b = direct(p.B, p.ldb, p.b_stride);
-  if (g.ta && !g.tb && p.n <= FEW_COLS && direct_a && direct_b && p.k % 8 == 0 && p.k > 0 &&
-      g.batch == 1 && g.tri == 0 && g.ep.scale == nullptr)
+  if (g.ta && !g.tb && p.n <= FEW_COLS && p.m <= FEW_ROWS && direct_a && direct_b &&
+      p.k % 8 == 0 && p.k > 0 && g.batch == 1 && g.tri == 0 && g.ep.scale == nullptr)
     return launch_few_columns<T>(h, p);
   const bool ring = (direct_a && direct_b) || pack_operands(h, g, p, direct_a, direct_b);
   // A lent workspace means that the library uses no memory of its own: nothing is cut.

@@ -456,6 +456,8 @@ Gemm16 step_product(int batch, int m, int n, int k, bool ta, bool tb, const void
 
 size_t newton_schulz_workspace_bytes(int m, int n, int batch) {
   if (m <= 0 || n <= 0 || batch <= 0 || is_small(m, n)) return 0;
+  // Twelve bytes an element bound the total from above, padding aside; no sum below wraps.
+  if (12.0 * batch * ((double)m + 64) * ((double)n + 64) > 0x1p60) return SIZE_MAX;
   return layout_of(m, n, batch).total + 256;
 }
 
@@ -482,9 +484,10 @@ rtat_status_t launch_newton_schulz(rtat_native_handle* h, int g_type, int m, int
     for (int i = 0; i < 3 * steps; ++i) q.coeffs[i] = coeffs[i];
     return m <= 64 && n <= 64 ? launch_small<64>(h, q, batch) : launch_small<128>(h, q, batch);
   }
+  const size_t bytes = newton_schulz_workspace_bytes(m, n, batch);
+  if (bytes == SIZE_MAX) return RTAT_STATUS_ALLOC_FAILED;
   const Layout l = layout_of(m, n, batch);
-  unsigned char* ws =
-      static_cast<unsigned char*>(acquire_workspace(h, newton_schulz_workspace_bytes(m, n, batch)));
+  unsigned char* ws = static_cast<unsigned char*>(acquire_workspace(h, bytes));
   if (ws == nullptr) return RTAT_STATUS_ALLOC_FAILED;
   ws = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ws) + 255) & ~(uintptr_t)255);
   uint16_t* const X[2] = {reinterpret_cast<uint16_t*>(ws), reinterpret_cast<uint16_t*>(ws + l.x1)};

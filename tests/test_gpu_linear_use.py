@@ -244,3 +244,19 @@ def test_update_batch_of_padded_rows(handle):
             want = ref.newton_schulz(g[:n * m].reshape(n, m), [QUINTIC] * 5)
             got = o[:n * m].reshape(n, m).double()
             assert ((got - want).norm() / want.norm()).item() <= 2.0 ** -9 + 3e-3
+
+
+def test_more_rows_than_a_launch_of_few_columns_holds(handle):
+    """A single column of more than 2^27 rows: two gigabytes of A."""
+    import torch
+    dt, ty = _types()["bf16"]
+    m, k = (1 << 27) + 17, 8
+    gen = _gen(6)
+    A = torch.randn(m, k, generator=gen, device="cuda", dtype=dt)
+    b = torch.randn(k, generator=gen, device="cuda", dtype=dt)
+    D = torch.full((m + 8,), float("nan"), device="cuda", dtype=dt)
+    handle.gemm_ep(ty, T, N, m, 1, k, 1.0, A, k, b, k, D, m)
+    assert torch.isnan(D[m:]).all()
+    for first in (0, 1 << 26, m - 5000):
+        y, e = ref.product(1.0, A[first:first + 5000], b[:, None], k)
+        assert _within(D[first:first + 5000, None], y, ref.rounded(y, e, dt))

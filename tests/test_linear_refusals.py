@@ -9,7 +9,7 @@ from rtatblas_amd import native
 
 BF16, F16, F32 = native.TYPE_BF16, native.TYPE_F16, native.TYPE_F32
 N, T = native.OP_N, native.OP_T
-OK, INVALID, UNSUPPORTED, NULL_HANDLE, ENUM = 0, 3, 7, 9, 10
+OK, ALLOC, INVALID, UNSUPPORTED, NULL_HANDLE, ENUM = 0, 2, 3, 7, 9, 10
 LONG = 2 ** 31 - 1000
 P = 4096                       # a pointer that is never followed
 
@@ -43,7 +43,8 @@ def ep(h, **kw):
     (dict(lda=3), INVALID), (dict(ldb=1), INVALID), (dict(ldd=3), INVALID), (dict(A=None), INVALID), (dict(B=None), INVALID),
     (dict(D=None), INVALID), (dict(ta=T, lda=1), INVALID), (dict(tb=T, ldb=2), INVALID), (dict(beta=1.0), INVALID),
     (dict(beta=1.0, C=P, ldc=3), INVALID), (dict(aux=P, ldaux=3), INVALID), (dict(m=0, D=None), OK), (dict(n=0, A=None), OK),
-    (dict(k=LONG, ldb=LONG), UNSUPPORTED), (dict(m=LONG, lda=LONG, ldd=LONG), UNSUPPORTED)])
+    (dict(k=LONG, ldb=LONG), UNSUPPORTED), (dict(m=LONG, lda=LONG, ldd=LONG), UNSUPPORTED),
+    (dict(n=2 ** 30 - 1023), UNSUPPORTED), (dict(n=2 ** 30 - 1024, D=None), INVALID)])
 def test_gemm_ep(bare, change, status):
     assert ep(bare, **change) == status
 
@@ -86,6 +87,7 @@ def test_dact(bare, change, status):
 @pytest.mark.parametrize("change,status", [
     (dict(g_type=5), ENUM), (dict(m=-1), INVALID), (dict(batch=-1), INVALID), (dict(coeffs=[]), INVALID),
     (dict(coeffs=[(1, 1, 1)] * 33), INVALID), (dict(eps=-1.0), INVALID), (dict(eps=float("nan")), INVALID), (dict(G=None), INVALID),
+    (dict(eps=float("inf")), INVALID), (dict(m=2 ** 30 - 1024, n=2 ** 30 - 1024, ldg=2 ** 30, ldo=2 ** 30), ALLOC),
     (dict(O=None), INVALID), (dict(ldg=3), INVALID), (dict(ldo=3), INVALID), (dict(batch=65536), INVALID), (dict(m=0, G=None), OK),
     (dict(n=LONG), UNSUPPORTED), (dict(n=0), OK), (dict(batch=0), OK)])
 def test_newton_schulz(bare, change, status):
@@ -102,4 +104,6 @@ def test_names_and_workspace_sizes():
     assert lib.rtat_newton_schulz_workspace_bytes(0, 4, 1) == 0
     one, six = (lib.rtat_newton_schulz_workspace_bytes(1000, 333, b) for b in (1, 6))
     # 1024 x 384 padded: two f16 and one f32 copy, and two 384 x 384 f16 matrices
+    assert lib.rtat_newton_schulz_workspace_bytes(2 ** 30 - 1024, 2 ** 30 - 1024, 1) == 2 ** 64 - 1
+    assert lib.rtat_newton_schulz_workspace_bytes(2 ** 30 - 1024, 2 ** 20, 65535) == 2 ** 64 - 1
     assert one >= 8 * 1024 * 384 + 4 * 384 * 384 and 5 * one < six <= 6 * one
