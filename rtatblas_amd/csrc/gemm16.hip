@@ -44,16 +44,19 @@ struct Gemm16Args {
 
 constexpr int BK16 = PANEL16;
 
-template <int BM_, int BN_, int WGM_, int WGN_, int OCC_, bool RING_ = false>
+template <int BM_, int BN_, int WGM_, int WGN_, int OCC_, int AHEAD_ = 0>
 struct Shape16 {
   static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, OCC = OCC_;
-  static constexpr bool RING = RING_;  // panels in a ring, accumulators of mfma_into
+  // Panels in a ring of SLOTS, AHEAD of A and of B there or on their way, accumulators of
+  // mfma_into; 0: two stages.
+  static constexpr int AHEAD = AHEAD_, SLOTS = AHEAD == 3 ? 8 : 5;
+  static constexpr bool RING = AHEAD > 0;
   static constexpr int NW = WGM * WGN, NT = 64 * NW;
   static constexpr int WTM = BM / WGM, WTN = BN / WGN;  // wave tile
   static constexpr int TM = WTM / 16, TN = WTN / 16;    // MFMA blocks per wave tile
   static constexpr int STAGE = (BM + BN) * BK16 * 2;    // bytes
   static constexpr int PARK = WTM + 4;                  // floats per parked column
-  static constexpr int LDS = RING_ ? 5 * BM * BK16 * 2 : 2 * STAGE;  // five panels, or two stages
+  static constexpr int LDS = RING ? SLOTS * BM * BK16 * 2 : 2 * STAGE;
   static_assert(LDS >= NW * 16 * PARK * 4, "room to park a block column per wave");
 };
 
@@ -108,6 +111,20 @@ struct Frags16 {
       const unsigned char* at = panel + base + step * 32 * P::ROWBYTES + (flip ^ (block * 32));
       const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(at));
       const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t)(at + 4 * P::ROWBYTES));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+  // The same with the panel's address in LDS: K-steps and halves (k-major: blocks) are offsets of
+  // the instruction, so an address serves several reads.
+  __device__ inline s8_t read_at(unsigned panel, int block, int step) const {
+    if constexpr (KMAJOR) {
+      typedef __attribute__((address_space(3))) const s8_t* lds8_t;
+      return ((lds8_t)(uintptr_t)(panel + base + (flip ^ (step * 64))))[block * P::ROWBYTES];
+    } else {
+      typedef __attribute__((address_space(3))) s4_t* lds4_t;
+      const lds4_t at = (lds4_t)(uintptr_t)(panel + base + (flip ^ (block * 32))) + step * 4 * P::ROWBYTES;
+      const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
+      const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at + P::ROWBYTES / 2);
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
@@ -557,6 +574,11 @@ template <int N>
 //     B in the second half (a slot that kt just left), eight loads in each half.  Loads are so
 //     evenly spread that a wave, alone on its SIMD, hardly waits to issue them (all sixteen in one
 //     half, into two 64 KiB stages: 8192^3 830 us; bunched at its start 865).
+//   * Smaller tiles run the same schedule, two or four workgroups a CU.  Where so few tiles are
+//     left that one or two a CU are all there is, a ring of eight slots keeps three panels on
+//     their way; a wave is then bound by issuing, and slot numbers modulo a power of two and one
+//     address for several reads leave 104 instructions to a panel instead of 150 (us at 64 x 64,
+//     1024^3: TN 8.0 -> 7.0, NT 11.0 -> 9.5; 128 x 128, 2048 x 2048 x 1024: NT 18.5 -> 15.7).
 //   * One barrier per panel, half way through it: by then the second half's operands are in
 //     registers, so both slots are free, and of the loads only the last eight may be missing.
 //   * Within a half the LDS reads of the next half and the panel loads are spread behind the
@@ -599,9 +621,11 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
                        ((!KA && !p.a_roomy && m0 + S::BM > p.m) ||
                         (!KB && !p.b_roomy && n0 + S::BN > p.n)));
   const int whole = panels - (ragged ? 1 : 0);
-  // Item 2 kt is A of panel kt, item 2 kt + 1 its B; item x lies in slot x % 5.
-  static_assert(S::BM == S::BN && S::LDS >= 5 * PA::BYTES, "slots of one size");
-  auto slot = [&](int item) { return lds + (item % 5) * PA::BYTES; };
+  // Item 2 kt is A of panel kt, item 2 kt + 1 its B; item x lies in slot x % SLOTS.
+  constexpr int AHEAD = S::AHEAD;
+  static_assert(AHEAD == 2 || AHEAD == 3, "the waits of the last panels");
+  static_assert(S::BM == S::BN && S::LDS >= S::SLOTS * PA::BYTES, "slots of one size");
+  auto slot = [&](int item) { return lds + (item % S::SLOTS) * PA::BYTES; };
   auto issue_all = [&](int kt) {
     if (kt < whole) {
       const u4_t pa = da.panel_at(At, p.lda, kt), pb = db.panel_at(Bt, p.ldb, kt);
@@ -627,8 +651,14 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
   s8_t fa[2][TM], fb[2][TN];
   // Operand x of a K-step, in the order the MFMAs want them: the first row of A, B, the other rows.
   auto read = [&](const unsigned char* pa, const unsigned char* pb, int step, int x) {
-    if (x == 0 || x > TN) fa[step][x == 0 ? 0 : x - TN] = ra.read(pa, x == 0 ? 0 : x - TN, step);
-    else fb[step][x - 1] = rb.read(pb, x - 1, step);
+    const int i = x == 0 ? 0 : x - TN;
+    if constexpr (S::BM == 256) {  // registers are short there, issue slots are not
+      if (x == 0 || x > TN) fa[step][i] = ra.read(pa, i, step);
+      else fb[step][x - 1] = rb.read(pb, x - 1, step);
+    } else {
+      if (x == 0 || x > TN) fa[step][i] = ra.read_at(lds_address(pa), i, step);
+      else fb[step][x - 1] = rb.read_at(lds_address(pb), x - 1, step);
+    }
   };
   // The MFMAs of one K-step, with read(x), x = 0 .. TM + TN - 1, spread behind the first three
   // quarters of them (as far as there are enough) and load(i), i = 0 .. NLOAD - 1, behind all.
@@ -658,20 +688,23 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
 
   if (panels > 0) {
     issue_all(0);
-    if (panels > 1) issue_all(1);
-    if (whole > 1) wait_and_meet<2 * NLOAD>();
+#pragma unroll
+    for (int i = 1; i < AHEAD; ++i)
+      if (i < panels) issue_all(i);
+    if (whole >= AHEAD) wait_and_meet<2 * NLOAD * (AHEAD - 1)>();
     else wait_and_meet<0>();
 #pragma unroll
     for (int x = 0; x < TM + TN; ++x) read(slot(0), slot(1), 0, x);
   }
   int kt = 0;
-  for (; kt < whole - 2; ++kt) {
+  for (; kt < whole - AHEAD; ++kt) {
     const unsigned char *a0 = slot(2 * kt), *b0 = slot(2 * kt + 1);
     const unsigned char *a1 = slot(2 * kt + 2), *b1 = slot(2 * kt + 3);
-    const u4_t pa = da.panel_at(At, p.lda, kt + 2), pb = db.panel_at(Bt, p.ldb, kt + 2);
-    const unsigned to_a = lds_address(slot(2 * kt + 4)), to_b = lds_address(a0);
+    const u4_t pa = da.panel_at(At, p.lda, kt + AHEAD), pb = db.panel_at(Bt, p.ldb, kt + AHEAD);
+    const unsigned to_a = lds_address(slot(2 * (kt + AHEAD)));
+    const unsigned to_b = lds_address(AHEAD == 2 ? a0 : slot(2 * (kt + AHEAD) + 1));
     multiply(0, [&](int x) { read(a0, b0, 1, x); }, [&](int i) { da.issue(i, pa, to_a, wave); });
-    wait_and_meet<NLOAD>();
+    wait_and_meet<NLOAD*(2 * AHEAD - 3)>();
     multiply(1, [&](int x) { read(a1, b1, 0, x); }, [&](int i) { db.issue(i, pb, to_b, wave); });
   }
 #pragma unroll 1
@@ -679,8 +712,9 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
     const unsigned char *a0 = slot(2 * kt), *b0 = slot(2 * kt + 1);
     const unsigned char *a1 = slot(2 * kt + 2), *b1 = slot(2 * kt + 3);
     multiply(0, [&](int x) { read(a0, b0, 1, x); }, no_load);
-    wait_and_meet<0>();
-    if (kt + 2 < panels) issue_all(kt + 2);
+    if (AHEAD == 3 && kt == whole - 3) wait_and_meet<2 * NLOAD>();  // panel kt + 2 is on its way
+    else wait_and_meet<0>();
+    if (kt + AHEAD < panels) issue_all(kt + AHEAD);
     multiply(1, [&](int x) { read(a1, b1, 0, x); }, no_load);  // of the last panel: not used
   }
   mfma_settle(acc);
@@ -689,9 +723,11 @@ __global__ __launch_bounds__(S::NT, S::OCC) void gemm16_dma_kernel(Gemm16Args p)
 #endif
 }
 
-typedef Shape16<256, 256, 2, 2, 1, true> S256x256;  // loads straight to LDS
-typedef Shape16<128, 128, 2, 2, 2, true> R128x128;
-typedef Shape16<64, 64, 2, 2, 4, true> R64x64;
+typedef Shape16<256, 256, 2, 2, 1, 2> S256x256;  // loads straight to LDS
+typedef Shape16<128, 128, 2, 2, 2, 2> R128x128;
+typedef Shape16<128, 128, 2, 2, 1, 3> D128x128;
+typedef Shape16<64, 64, 2, 2, 4, 2> R64x64;
+typedef Shape16<64, 64, 2, 2, 2, 3> D64x64;
 typedef Shape16<128, 128, 2, 2, 2> S128x128;  // any alignment
 typedef Shape16<64, 64, 2, 2, 4> S64x64;
 
@@ -1046,6 +1082,14 @@ rtat_status_t launch_type(rtat_native_handle* h, const Gemm16& g, Gemm16Args p) 
     return plan.tile == 128 ? launch_ops16<T, S128x128, false>(h, g, p)
                             : launch_ops16<T, S64x64, false>(h, g, p);
   if (plan.tile == 256) return launch_ops16<T, S256x256, true>(h, g, p);
+  // With one 128 x 128 tile a CU, or two of 64 x 64, there is room for the longer ring.
+  const long cus = h->compute_units > 0 ? h->compute_units : 256;
+  const long side_m = (p.m + plan.tile - 1) / plan.tile, side_n = (p.n + plan.tile - 1) / plan.tile;
+  const long tiles = (plan.tri ? side_m * (side_m + 1) / 2 : side_m * side_n) *
+                     (plan.slices > 1 ? plan.slices : g.batch);
+  if (tiles <= (plan.tile == 128 ? 1 : 2) * cus)
+    return plan.tile == 128 ? launch_ops16<T, D128x128, true>(h, g, p)
+                            : launch_ops16<T, D64x64, true>(h, g, p);
   return plan.tile == 128 ? launch_ops16<T, R128x128, true>(h, g, p)
                           : launch_ops16<T, R64x64, true>(h, g, p);
 }

@@ -6,12 +6,12 @@
 // launches of 16 .. 2048 tiles with 16 .. 128 panels (64 elements of k) on 256 CUs, in us:
 //   256 x 256   8 + 1.25 a panel, per round of one tile a CU
 //   128 x 128   4.3 per round of two, and a panel 0.44 per tile of a CU, 0.5 at least
-//    64 x 64    3.7 per round of four, and a panel 0.175 per tile of a CU, 0.4 at least
+//    64 x 64    3.7 per round of four, and a panel 0.175 per tile of a CU, 0.3 at least
 //   slices      3 for the second launch, and their bytes, written and read once, at 4 MB/us
 //   the mirrored half of a symmetric product: 7 (narrow stores), 3 when slices are joined
 // Examples (us, chosen / the other shapes whole): 4096 x 2048 x 2048 128: 33 / 64: 52, 256: 49;
-// 2048 x 3584 x 4096 128: 61 / 83, 82; 1024^3 64: 7.5 / 128: 11, 256: 25; 768 x 768 x 8192 in
-// slices 25 / 46, 59, 141.
+// 2048 x 3584 x 4096 128: 61 / 83, 82; 1024^3 64: 6.5 / 128: 11, 256: 25; 768 x 768 x 8192 in
+// slices 23 / 46, 59, 141.
 #pragma once
 #include <stddef.h>
 
@@ -33,7 +33,7 @@ inline double price16(int tile, long tiles, long panels, long cus) {
   const long w = (tiles + cus - 1) / cus;  // tiles of the busiest CU
   const double p = (double)panels;
   if (tile == 256) return (double)w * (8.0 + 1.25 * p);
-  const double per = tile == 128 ? 0.44 : 0.175, least = tile == 128 ? 0.5 : 0.4;
+  const double per = tile == 128 ? 0.44 : 0.175, least = tile == 128 ? 0.5 : 0.3;
   const double fixed = tile == 128 ? 4.3 * (double)((w + 1) / 2) : 3.7 * (double)((w + 3) / 4);
   const double panel = per * (double)w > least ? per * (double)w : least;
   return fixed + panel * p;
