@@ -986,20 +986,28 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
   const PackJob j = p.job[blockIdx.y];
   const int lane = threadIdx.x % 32, first = blockIdx.x * PACK_COLS + threadIdx.x / 32;
   for (int row = (blockIdx.z * 32 + lane) * 8; row < j.ldd; row += gridDim.z * 256) {
+    const uint16_t* const at = j.src + (long)first * j.ld + row;
+    s8_t v[PACK_COLS / 8];
+    // Inside, all loads are on their way before the first is waited for.
+    if (row + 8 <= j.rows && first + PACK_COLS - 8 < j.cols) {
 #pragma unroll
-    for (int c = 0; c < PACK_COLS; c += 8) {
-      const int col = first + c;
-      if (col >= j.cols_out) continue;
-      const uint16_t* at = j.src + (long)col * j.ld + row;
-      s8_t v = {};
-      if (col < j.cols && row + 8 <= j.rows) {
-        v = __builtin_bit_cast(s8_t, load16(at, 0));
-      } else if (col < j.cols) {
+      for (int c = 0; c < PACK_COLS / 8; ++c)
+        v[c] = __builtin_bit_cast(s8_t, load16(at + 8L * c * j.ld, 0));
+    } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = row + e < j.rows ? (short)at[e] : (short)0;
+      for (int c = 0; c < PACK_COLS / 8; ++c) {
+        v[c] = s8_t{};
+        if (first + 8 * c < j.cols) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (row + e < j.rows) v[c][e] = (short)at[8L * c * j.ld + e];
+        }
       }
-      *reinterpret_cast<s8_t*>(j.dst + (long)col * j.ldd + row) = v;
     }
+#pragma unroll
+    for (int c = 0; c < PACK_COLS / 8; ++c)
+      if (first + 8 * c < j.cols_out)
+        *reinterpret_cast<s8_t*>(j.dst + (first + 8L * c) * j.ldd + row) = v[c];
   }
 }
 
