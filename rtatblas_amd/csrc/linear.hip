@@ -5,7 +5,10 @@
 // lanes take 128 neighbouring rows of a column in 16-byte accesses, a workgroup of 256 sixteen
 // columns at a time; the columns are cut into chunks so that the grid fills the machine, each
 // chunk leaves one row of partial sums and a second small launch adds those in order, so the
-// result does not depend on timing.
+// result does not depend on timing.  Four groups of columns on their way before the first store:
+// 6580 x 4711 f16 on 8-byte aligned columns 62 -> 47 us, 413 x 456 20 -> 12.
+#include <type_traits>
+
 #include "gemm16.h"
 
 namespace rtat_native {
@@ -13,6 +16,7 @@ namespace rtat_native {
 namespace {
 
 constexpr int ROWS = 128, COLS = 16;  // rows and columns a workgroup holds at a time
+constexpr int AHEAD = 4;              // that many times COLS are on their way
 
 struct ActArgs {
   int type, act, m, n, per_chunk;
@@ -25,6 +29,19 @@ struct ActArgs {
   float* sums;  // [chunk][m], or null
 };
 
+// Eight neighbours, of which the first `left` >= 1 are there; the others read as zero.  Without
+// branches, so that loads of several columns overlap.
+template <bool PART>
+__device__ inline u4_t fetch8(const uint16_t* p, long i, int left) {
+  if (!PART) return load16(p, 2 * i);
+  s8_t v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (short)p[i + (e < left ? e : left - 1)];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = e < left ? v[e] : (short)0;
+  return __builtin_bit_cast(u4_t, v);
+}
+
 __global__ __launch_bounds__(256) void act_backward_kernel(ActArgs p) {
   __shared__ float part[COLS][ROWS];
   const int t = threadIdx.x, lr = (t % 16) * 8, lc = t / 16;
@@ -35,35 +52,39 @@ __global__ __launch_bounds__(256) void act_backward_kernel(ActArgs p) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) sums[i] = 0.0f;
   const bool slope = p.act != RTAT_ACT_NONE;
-  if (row < p.m) {
-    if (row + 8 <= p.m) {
-#pragma unroll 4
-      for (int col = first + lc; col < last; col += COLS) {
+  const int left = p.m - row;
+  auto columns = [&](auto part) {
+    constexpr bool PART = decltype(part)::value;
+    // Four columns are asked for before the first is stored: dZ may be dD, so the compiler would
+    // not move a load over a store by itself.
+    for (int col = first + lc; col < last; col += AHEAD * COLS) {
+      u4_t d[AHEAD], z[AHEAD][1];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int c = col + u * COLS < last ? col + u * COLS : last - 1;  // its sums are left out
+        d[u] = fetch8<PART>(p.dD, row + (long)c * p.lddd, left);
+        z[u][0] = slope ? fetch8<PART>(p.Z, row + (long)c * p.ldz, left) : u4_t{};
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int c = col + u * COLS;
+        if (c >= last) break;
         float v[1][8];
-        load8(p.type, p.dD, row + (long)col * p.lddd, v[0]);
+        unpack8(p.type, d[u], v[0]);
         if (slope) {
-          const u4_t z[1] = {load16(p.Z, 2 * (row + (long)col * p.ldz))};
-          act_slopes<1>(p.act, p.type, z, v);
-          if (p.dZ != nullptr) store8(p.type, p.dZ, row + (long)col * p.lddz, v[0]);
+          act_slopes<1>(p.act, p.type, z[u], v);
+          if (p.dZ != nullptr) {
+            if (PART) store8_part(p.type, p.dZ, row + (long)c * p.lddz, left, v[0]);
+            else store8(p.type, p.dZ, row + (long)c * p.lddz, v[0]);
+          }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) sums[i] += v[0][i];
       }
-    } else {
-      for (int col = first + lc; col < last; col += COLS) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (row + i < p.m) {
-            float v = load_one(p.type, p.dD, row + i + (long)col * p.lddd);
-            if (slope) {
-              v *= act_slope(p.act, load_one(p.type, p.Z, row + i + (long)col * p.ldz));
-              if (p.dZ != nullptr) store_one(p.type, p.dZ, row + i + (long)col * p.lddz, v);
-            }
-            sums[i] += v;
-          }
-      }
     }
-  }
+  };
+  if (left >= 8) columns(std::false_type());
+  else if (left > 0) columns(std::true_type());
   if (p.sums == nullptr) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) part[lc][lr + i] = sums[i];
