@@ -260,3 +260,22 @@ def test_more_rows_than_a_launch_of_few_columns_holds(handle):
     for first in (0, 1 << 26, m - 5000):
         y, e = ref.product(1.0, A[first:first + 5000], b[:, None], k)
         assert _within(D[first:first + 5000, None], y, ref.rounded(y, e, dt))
+
+
+@pytest.mark.parametrize("side", [72, 1600, 2048, 2304])
+@pytest.mark.parametrize("ops", [(T, N), (N, N), (N, T), (T, T)])
+def test_any_number_of_panels(handle, side, ops):
+    """From part of one panel of k to more than any ring of panels holds, whole and not, at sides
+    that run on different tiles, with NaN behind every column of the operands."""
+    import torch
+    dt, ty = _types()["bf16"]
+    gen = _gen(side)
+    D = Mat(side, side, dt, 8)
+    for k in (8, 56, 64, 72, 128, 136, 192, 200, 256, 264, 320, 328, 384, 440, 576):
+        shapes = [(side, k) if op == N else (k, side) for op in (ops[0], ops[1])]
+        shapes[1] = (k, side) if ops[1] == N else (side, k)
+        A, B = (Mat(r, c, dt, 8, 0, gen) for r, c in shapes)
+        handle.gemm_ep(ty, *ops, side, side, k, 1.0, A.ptr, A.ld, B.ptr, B.ld, D.ptr, D.ld)
+        a, b = A.m if ops[0] == N else A.m.T, B.m if ops[1] == N else B.m.T
+        y, e = ref.product(1.0, a, b, k)
+        assert _within(D.m, y, ref.rounded(y, e, dt)) and D.padding_kept(), k
