@@ -375,9 +375,14 @@ size_t rtat_dbias_workspace_bytes(int m, int n);
  *   M = X X^T,  X = a X + (b M + c M^2) X;   O = X
  * (for m > n the same with M = X^T X).  coeffs is a host array of 3 * steps floats, read before
  * the call returns; 1 <= steps <= RTAT_NEWTON_SCHULZ_MAX_STEPS, batch <= 65535 and eps finite and
- * not negative (else RTAT_STATUS_INVALID_VALUE).  Between products X and M are
- * held in f16, scaled so that singular values up to 60 of X fit, and X in f32 as well until the
- * last two steps, so O carries about nine bits: that is why it is BF16 whatever g_type is.
+ * not negative (else RTAT_STATUS_INVALID_VALUE).
+ * Between products X, M and b M + c M^2 are held in f16, and X in f32 as well until the last two
+ * steps.  Singular values of X up to 60 before a step fit, whatever the coefficients; beyond that
+ * O holds infinities or NaN.  (Before the first step they are at most 1; the last step may take
+ * them anywhere.)  With convergent coefficients O carries about nine bits of its norm: that is why
+ * it is BF16 whatever g_type is.  A rounding, 2^-12 of the largest singular value, grows by `a` in
+ * every later step, so where G is singular O has an error of about that times the product of the
+ * later a's, and elements below 2^-34 of ||G_i|| + eps count as zero.
  * G_i = G + i * stride_g, O_i = O + i * stride_o (elements; ignored when batch <= 1); O may be G
  * when g_type is BF16 and the leading dimensions and strides agree.  An infinity or a NaN in G_i
  * makes O_i NaN throughout and no other.

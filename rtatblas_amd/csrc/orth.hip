@@ -14,9 +14,11 @@
 // products unchanged and every operand aligned.
 //
 // Precision.  X and M are f16 (11 bits) rather than bf16 (8): both run at the same rate, and all
-// values are bounded, so a fixed scale keeps them in range: X by 2^10 (|x| <= singular value, so
-// up to 60 fits; entries of size 2^-24 relative to the norm are still normal numbers), M by 2^10,
-// b M + c M^2 by 2^8.  A rounding of X in an early step is amplified by a^(steps left) in weak
+// values are bounded, so scales keep them in range: X by 2^10 (|x| <= singular value, so up to 60
+// fits; the norm of the first X lies in (512, 1024], so entries down to 2^-24 of it are within a
+// factor of two of f16's smallest normal number), M by at most 2^10 and b M + c M^2 by at most 2^8, as far
+// as a bound on the singular values leaves room (orth_plan.h).
+// A rounding of X in an early step is amplified by a^(steps left) in weak
 // directions, so early steps add a X from an f32 copy (or from a 16-bit G, which f16 holds
 // exactly); in the last two, where singular values have grown to the order of one, a joins the
 // diagonal of the polynomial instead.  Relative error of the result in 2-norm against 64 bits,
@@ -26,12 +28,12 @@
 // The norm is summed in f64.  G is scaled by a power of two when it becomes f16, so a 16-bit G
 // does not round; what is left of the norm (r in [1, 2)) enters the scalars of step 0.
 #include "gemm16.h"
+#include "orth_plan.h"
 
 namespace rtat_native {
 
 namespace {
 
-constexpr float X_SCALE = 1024.0f, M_SCALE = 1024.0f, P_SCALE = 256.0f;
 constexpr int NORM_BLOCKS = 1024;  // partial sums per matrix, at most
 
 struct NormArgs {
@@ -196,7 +198,7 @@ struct SmallArgs {
   int steps;
   uint16_t* O;
   long ldo, stride_o;
-  float coeffs[3 * RTAT_NEWTON_SCHULZ_MAX_STEPS];
+  StepFactors step[RTAT_NEWTON_SCHULZ_MAX_STEPS];
 };
 
 template <int SIDE>
@@ -327,33 +329,32 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(SmallArgs p) {
   f4_t acc[TM][TN];
 #pragma unroll 1
   for (int step = 0; step < p.steps; ++step) {
-    const float ca = p.coeffs[3 * step], cb = p.coeffs[3 * step + 1], cc = p.coeffs[3 * step + 2];
+    const StepFactors& k = p.step[step];
     const float f = step == 0 ? r : 1.0f;
     const bool adds = step < p.steps - 2, last = step == p.steps - 1;
     Q::template multiply<false>(X, X, m0, n0, lane, acc);  // M = X^T X
-    const float am = f * f * (M_SCALE / (X_SCALE * X_SCALE));
+    const float am = f * f * k.m;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) Q::put(M, lo0 + 16 * j, hi0 + 16 * i, acc[i][j] * am);
     __syncthreads();
     Q::template multiply<false>(M, M, m0, n0, lane, acc);  // P = b M + c M^2 (+ a)
-    const float ap = cc * (P_SCALE / (M_SCALE * M_SCALE)), bp = cb * (P_SCALE / M_SCALE);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         const int row = hi0 + 16 * i, col = lo0 + 16 * j;
-        f4_t w = acc[i][j] * ap + Q::get(M, col, row) * bp;
+        f4_t w = acc[i][j] * k.p + Q::get(M, col, row) * k.q;
         if (!adds) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) w[q] += row + q == col ? ca * P_SCALE : 0.0f;
+          for (int q = 0; q < 4; ++q) w[q] += row + q == col ? k.diag : 0.0f;
         }
         Q::put(P, col, row, w);
       }
     __syncthreads();
     Q::template multiply<true>(X, P, m0, n0, lane, acc);  // X P (+ a X)
-    const float ax = f / P_SCALE, bx = ca * f;
+    const float ax = f * k.back, bx = k.a * f;
     __syncthreads();  // X has been read
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -481,7 +482,7 @@ rtat_status_t launch_newton_schulz(rtat_native_handle* h, int g_type, int m, int
     q.O = static_cast<uint16_t*>(O);
     q.ldo = ldo;
     q.stride_o = stride_o;
-    for (int i = 0; i < 3 * steps; ++i) q.coeffs[i] = coeffs[i];
+    step_factors(steps, coeffs, q.step);
     return m <= 64 && n <= 64 ? launch_small<64>(h, q, batch) : launch_small<128>(h, q, batch);
   }
   const size_t bytes = newton_schulz_workspace_bytes(m, n, batch);
@@ -528,14 +529,16 @@ rtat_status_t launch_newton_schulz(rtat_native_handle* h, int g_type, int m, int
   st = launch_status();
   if (st != RTAT_STATUS_SUCCESS) return st;
 
+  StepFactors factors[RTAT_NEWTON_SCHULZ_MAX_STEPS];
+  step_factors(steps, coeffs, factors);
   for (int i = 0; i < steps; ++i) {
-    const float ca = coeffs[3 * i], cb = coeffs[3 * i + 1], cc = coeffs[3 * i + 2];
+    const StepFactors& k = factors[i];
     const bool last = i == steps - 1;
     const uint16_t* const x = X[i & 1];
     uint16_t* const y = X[(i + 1) & 1];
     // M = X^T X
-    Gemm16 g = step_product(batch, lp, lp, hp, true, false, x, hp, xs, x, hp, xs,
-                            M_SCALE / (X_SCALE * X_SCALE), M, lp, ps, RTAT_TYPE_F16);
+    Gemm16 g = step_product(batch, lp, lp, hp, true, false, x, hp, xs, x, hp, xs, k.m,
+                            M, lp, ps, RTAT_TYPE_F16);
     g.tri = 1;
     if (i == 0) {
       g.ep.scale = scale;
@@ -544,24 +547,24 @@ rtat_status_t launch_newton_schulz(rtat_native_handle* h, int g_type, int m, int
     st = launch_gemm16(h, g);
     if (st != RTAT_STATUS_SUCCESS) return st;
     // P = b M + c M^2 (+ a)
-    g = step_product(batch, lp, lp, lp, true, false, M, lp, ps, M, lp, ps,
-                     cc * P_SCALE / (M_SCALE * M_SCALE), P, lp, ps, RTAT_TYPE_F16);
+    g = step_product(batch, lp, lp, lp, true, false, M, lp, ps, M, lp, ps, k.p, P,
+                     lp, ps, RTAT_TYPE_F16);
     g.tri = 1;
-    g.ep.beta = cb * P_SCALE / M_SCALE;
+    g.ep.beta = k.q;
     g.ep.C = M;
     g.ep.ldc = lp;
     g.ep.c_stride = ps;
     g.ep.c_type = RTAT_TYPE_F16;
-    g.ep.diag = adds(i) ? 0.0f : ca * P_SCALE;
+    g.ep.diag = k.diag;
     st = launch_gemm16(h, g);
     if (st != RTAT_STATUS_SUCCESS) return st;
     // X = X P (+ a X)
     if (!last) {
-      g = step_product(batch, hp, lp, lp, false, false, x, hp, xs, P, lp, ps, 1.0f / P_SCALE, y, hp,
+      g = step_product(batch, hp, lp, lp, false, false, x, hp, xs, P, lp, ps, k.back, y, hp,
                        xs, RTAT_TYPE_F16);
       if (adds(i)) {
         const bool f32 = i > 0 || a.F != nullptr;
-        g.ep.beta = ca;
+        g.ep.beta = k.a;
         g.ep.C = f32 ? static_cast<const void*>(F) : x;
         g.ep.ldc = hp;
         g.ep.c_stride = xs;
@@ -575,11 +578,11 @@ rtat_status_t launch_newton_schulz(rtat_native_handle* h, int g_type, int m, int
         g.ep.d_type = RTAT_TYPE_F32;
       }
     } else if (turn) {  // O = (X P)^T = P X^T
-      g = step_product(batch, m, n, lp, true, true, P, lp, ps, x, hp, xs, 1.0f / (P_SCALE * X_SCALE),
+      g = step_product(batch, m, n, lp, true, true, P, lp, ps, x, hp, xs, k.back / X_SCALE,
                        O, ldo, stride_o, RTAT_TYPE_BF16);
     } else {
       g = step_product(batch, m, n, lp, false, false, x, hp, xs, P, lp, ps,
-                       1.0f / (P_SCALE * X_SCALE), O, ldo, stride_o, RTAT_TYPE_BF16);
+                       k.back / X_SCALE, O, ldo, stride_o, RTAT_TYPE_BF16);
     }
     if (i == 0) {
       g.ep.scale = scale;
