@@ -175,16 +175,22 @@ def _plain_orth(s, case):
 # ---- the same through the library --------------------------------------------------------
 
 _lib = {}
+_handles = {}
 
 
 def _handle():
-    """The program's one handle, on torch's current stream."""
+    """The program's handle on torch's current stream.  A handle works on one stream, its scratch with it, so every stream has
+    one of its own; a stream that is to be captured runs a pass first, which creates it."""
     if not _lib:
         from rtatblas_amd import native
-        _lib["native"], _lib["handle"] = native, native.Handle(torch.cuda.current_stream())
+        _lib["native"] = native
         _lib["type"] = {torch.bfloat16: native.TYPE_BF16, torch.float16: native.TYPE_F16, torch.float32: native.TYPE_F32}
         _lib["act"] = {a: getattr(native, "ACT_" + a.upper()) for a in ACTS}
-    return _lib["native"], _lib["handle"]
+    stream = torch.cuda.current_stream()
+    on = (stream.device_index, stream.cuda_stream)
+    if on not in _handles:
+        _handles[on] = _lib["native"].Handle(stream)
+    return _lib["native"], _handles[on]
 
 
 def _own_fwd(s, case, dt):
