@@ -72,19 +72,23 @@ struct __attribute__((packed, aligned(2))) Loose16 {
 __device__ inline float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896f); }
 __device__ inline float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// Phi(z) and the density phi(z) of the normal distribution.  erfc by Abramowitz and Stegun 7.1.26
-// (a quintic in t = 1 / (1 + p x) times exp(-x^2), off by at most 1.5e-7), x = |z| / sqrt 2, so
-// that one exponential serves both.
+// Phi(z) and the density phi(z) of the normal distribution.  The tail beyond a = |z| is exp(-a^2 / 2)
+// times t q(t), t = 1 / (1 + 0.305 a): a septic fitted for the least largest relative error (9.4e-8
+// over 0 <= a <= 14), so that one exponential serves both and small values of z Phi(z) keep their
+// leading bits: relative to the tail at most 6.2 half steps of f32 times 1 + a^2, emulated, from
+// rounding a^2.  Exactly a half at 0.
 __device__ inline void normal_cdf(float z, float& Phi, float& phi) {
-  const float x = __builtin_fabsf(z) * 0.707106781186548f;
-  const float e = exp_fast(-x * x);
-  const float t = rcp_fast(__builtin_fmaf(0.3275911f, x, 1.0f));
-  float q = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-  q = __builtin_fmaf(q, t, 1.421413741f);
-  q = __builtin_fmaf(q, t, -0.284496736f);
-  q = __builtin_fmaf(q, t, 0.254829592f);
-  const float half_erfc = 0.5f * q * t * e;
-  Phi = z < 0.0f ? half_erfc : 1.0f - half_erfc;
+  const float e = __builtin_amdgcn_exp2f(z * z * -0.721347520444482f);
+  const float t = rcp_fast(__builtin_fmaf(0.305f, __builtin_fabsf(z), 1.0f));
+  float q = __builtin_fmaf(0.0366991985f, t, -0.152988333f);
+  q = __builtin_fmaf(q, t, 0.185716919f);
+  q = __builtin_fmaf(q, t, -0.0379768468f);
+  q = __builtin_fmaf(q, t, 0.121021689f);
+  q = __builtin_fmaf(q, t, 0.103420865f);
+  q = __builtin_fmaf(q, t, 0.12246682f);
+  q = __builtin_fmaf(q, t, 0.121639735f);
+  const float tail = q * t * e;
+  Phi = z < 0.0f ? tail : 1.0f - tail;
   phi = 0.398942280401433f * e;
 }
 
