@@ -20,23 +20,21 @@ def ops():
 def test_a_handle_for_every_stream(ops, monkeypatch):
     from rtatblas_amd import native
 
-    class Stream:
-        def __init__(self, device, raw):
-            self.device_index, self.cuda_stream = device, raw
-
     class Handle:
         def __init__(self, stream):
-            self.on = (stream.device_index, stream.cuda_stream)
+            self.stream = stream
 
     now = []
-    monkeypatch.setattr(ops.torch.cuda, "current_stream", lambda: now[-1])
+    monkeypatch.setattr(ops.torch.cuda, "current_device", lambda: now[-1][0])
+    monkeypatch.setattr(ops.torch._C, "_cuda_getCurrentRawStream", lambda device: now[-1][1] if device == now[-1][0] else None)
     monkeypatch.setattr(native, "Handle", Handle)
     seen = {}
     for on in [(0, 0), (0, 64), (0, 0), (1, 0), (0, 64), (1, 64)]:
-        now.append(Stream(*on))
+        now.append(on)
         h = ops._handle()[1]
-        assert h.on == on
+        assert h.stream == on[1]
         assert seen.setdefault(on, h) is h
+    assert len({id(h) for h in seen.values()}) == 4
 
 
 CASES = [
