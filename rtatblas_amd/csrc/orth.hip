@@ -426,13 +426,14 @@ Layout layout_of(int m, int n, int batch) {
   return l;
 }
 
-// One product of a step on matrices of the scratch.
-Gemm16 step_product(int batch, int m, int n, int k, bool ta, bool tb, const void* A, long lda,
+// One product of a step on matrices of the scratch, of which `used` bytes are the iteration's.
+Gemm16 step_product(size_t used, int batch, int m, int n, int k, bool ta, bool tb, const void* A, long lda,
                     long a_stride, const void* B, long ldb, long b_stride, float alpha, void* D,
                     long ldd, long d_stride, int d_type) {
   Gemm16 g = {};
   g.type = RTAT_TYPE_F16;
   g.batch = batch;
+  g.scratch_used = used;
   g.m = g.ep.rows = m;
   g.n = g.ep.cols = n;
   g.k = k;
@@ -537,7 +538,7 @@ rtat_status_t launch_newton_schulz(rtat_native_handle* h, int g_type, int m, int
     const uint16_t* const x = X[i & 1];
     uint16_t* const y = X[(i + 1) & 1];
     // M = X^T X
-    Gemm16 g = step_product(batch, lp, lp, hp, true, false, x, hp, xs, x, hp, xs, k.m,
+    Gemm16 g = step_product(bytes, batch, lp, lp, hp, true, false, x, hp, xs, x, hp, xs, k.m,
                             M, lp, ps, RTAT_TYPE_F16);
     g.tri = 1;
     if (i == 0) {
@@ -547,7 +548,7 @@ rtat_status_t launch_newton_schulz(rtat_native_handle* h, int g_type, int m, int
     st = launch_gemm16(h, g);
     if (st != RTAT_STATUS_SUCCESS) return st;
     // P = b M + c M^2 (+ a)
-    g = step_product(batch, lp, lp, lp, true, false, M, lp, ps, M, lp, ps, k.p, P,
+    g = step_product(bytes, batch, lp, lp, lp, true, false, M, lp, ps, M, lp, ps, k.p, P,
                      lp, ps, RTAT_TYPE_F16);
     g.tri = 1;
     g.ep.beta = k.q;
@@ -560,7 +561,7 @@ rtat_status_t launch_newton_schulz(rtat_native_handle* h, int g_type, int m, int
     if (st != RTAT_STATUS_SUCCESS) return st;
     // X = X P (+ a X)
     if (!last) {
-      g = step_product(batch, hp, lp, lp, false, false, x, hp, xs, P, lp, ps, k.back, y, hp,
+      g = step_product(bytes, batch, hp, lp, lp, false, false, x, hp, xs, P, lp, ps, k.back, y, hp,
                        xs, RTAT_TYPE_F16);
       if (adds(i)) {
         const bool f32 = i > 0 || a.F != nullptr;
@@ -578,10 +579,10 @@ rtat_status_t launch_newton_schulz(rtat_native_handle* h, int g_type, int m, int
         g.ep.d_type = RTAT_TYPE_F32;
       }
     } else if (turn) {  // O = (X P)^T = P X^T
-      g = step_product(batch, m, n, lp, true, true, P, lp, ps, x, hp, xs, k.back / X_SCALE,
+      g = step_product(bytes, batch, m, n, lp, true, true, P, lp, ps, x, hp, xs, k.back / X_SCALE,
                        O, ldo, stride_o, RTAT_TYPE_BF16);
     } else {
-      g = step_product(batch, m, n, lp, false, false, x, hp, xs, P, lp, ps,
+      g = step_product(bytes, batch, m, n, lp, false, false, x, hp, xs, P, lp, ps,
                        k.back / X_SCALE, O, ldo, stride_o, RTAT_TYPE_BF16);
     }
     if (i == 0) {
