@@ -1,7 +1,8 @@
-// Host tests of the linear-layer operators' planning headers (orth_plan.h).
+// Host tests of the linear-layer operators' planning headers (orth_plan.h, gemm16_plan.h).
 #include <cmath>
 #include <vector>
 #include "mini_test.h"
+#include "gemm16_plan.h"
 #include "orth_plan.h"
 
 using namespace rtat_native;
@@ -83,4 +84,49 @@ TEST(orth_plan, scales_stay_finite_for_any_coefficients, false) {
       CHECK(x.m >= 16.0f / 1048576.0f && x.back >= 1.0f / 256.0f && x.back <= 0x1p120f);
     }
   }
+}
+
+// ---- gemm16_plan.h -------------------------------------------------------------------------
+
+TEST(gemm16_plan, choices_that_were_measured, false) {
+  const size_t scratch = (size_t)64 << 20;
+  struct Case {
+    int m, n, k, tile;
+    bool cut;
+  };
+  for (const Case& c : {Case{4096, 2048, 2048, 128, false}, Case{2048, 3584, 4096, 128, false},
+                        Case{1024, 1024, 1024, 64, false}, Case{768, 768, 8192, 64, true},
+                        Case{8192, 8192, 8192, 256, false}, Case{8192, 8192, 4096, 256, false}}) {
+    const Plan16 p = plan16(c.m, c.n, c.k, 1, false, true, scratch, 256);
+    CHECK_EQ(p.tri, 0);
+    CHECK_EQ(p.slices > 1, c.cut);
+    if (!c.cut) CHECK_EQ(p.tile, c.tile);
+  }
+  // The smaller half of a symmetric product, where its tiles fill the machine.
+  CHECK_EQ(plan16(8192, 8192, 8192, 1, true, true, scratch, 256).tri, 1);
+}
+
+// What the kernels index by: slices have panels and room, halves only where they are asked for, the
+// join's grid within its limit.
+TEST(gemm16_plan, whatever_is_chosen_fits, false) {
+  const int sizes[] = {1, 7, 16, 63, 64, 65, 129, 333, 512, 1000, 2051, 4099, 8192, 1 << 20, (1 << 30) - 1024};
+  for (int m : sizes)
+    for (int n : sizes)
+      for (int k : {0, 1, 64, 65, 1000, 8192, 1 << 20})
+        for (int batch : {1, 6})
+          for (int symmetric = 0; symmetric <= (m == n ? 1 : 0); ++symmetric)
+            for (int large : {0, 1})
+              for (size_t scratch : {(size_t)0, (size_t)1 << 20, (size_t)64 << 20}) {
+                const Plan16 p = plan16(m, n, k, batch, symmetric != 0, large != 0, scratch, 256);
+                const long panels = ((long)k + PANEL16 - 1) / PANEL16;
+                CHECK(p.tile == 64 || p.tile == 128 || (p.tile == 256 && large));
+                CHECK(p.tri == 0 || symmetric);
+                CHECK(p.slices >= 1 && p.slices <= 64);
+                if (p.slices > 1) {
+                  CHECK(batch == 1 && panels / p.slices >= SLICE_PANELS16);
+                  CHECK((double)p.slices * slice_ld16(m) * n * 4.0 <= (double)scratch);
+                  CHECK(p.tri == 0 || p.tile == 128);
+                  CHECK(((long)n + 15) / 16 <= 65535);
+                }
+              }
 }
