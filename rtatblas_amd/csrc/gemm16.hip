@@ -870,8 +870,7 @@ bool direct(const void* base, long ld, long stride) {
 // waves' sums meet in LDS.  Sixteen waves read deep enough that 128 workgroups keep memory busy,
 // so nothing is cut across workgroups.  Measured (us; 64 x 64 tiles in slices in brackets):
 // 8192 x 1 x 2048 5.9 (10.9), 2048 x 13 x 8192 9.2 (13.2), 8192 x 16 x 8192 22 (35).
-constexpr int FEW_COLS = 16, FEW_DEEP = 8, FEW_WAVES = 16;
-constexpr int FEW_ROWS = 1 << 27;  // 2^23 workgroups of 256: a launch holds fewer than 2^32 threads
+constexpr int FEW_DEEP = 8, FEW_WAVES = 16;
 
 template <class T>
 __global__ __launch_bounds__(64 * FEW_WAVES) void few_columns_kernel(Gemm16Args p) {
@@ -1076,12 +1075,12 @@ bool pack_operands(rtat_native_handle* h, const Gemm16& g, Gemm16Args& p, bool d
 template <class T>
 rtat_status_t launch_type(rtat_native_handle* h, const Gemm16& g, Gemm16Args p) {
   const bool direct_a = direct(p.A, p.lda, p.a_stride), direct_b = direct(p.B, p.ldb, p.b_stride);
-  if (g.ta && !g.tb && p.n <= FEW_COLS && p.m <= FEW_ROWS && direct_a && direct_b &&
-      p.k % 8 == 0 && p.k > 0 && g.batch == 1 && g.tri == 0 && g.ep.scale == nullptr)
-    return launch_few_columns<T>(h, p);
-  const bool ring = (direct_a && direct_b) || pack_operands(h, g, p, direct_a, direct_b);
   // A lent workspace means that the library uses no memory of its own: nothing is cut.
   const size_t scratch = h->user_ws == nullptr && h->split_ws != nullptr ? SPLIT_WS_BYTES : 0;
+  if (g.ta && !g.tb && direct_a && direct_b && few_columns16(p.m, p.n, p.k, scratch) && g.batch == 1 &&
+      g.tri == 0 && g.ep.scale == nullptr)
+    return launch_few_columns<T>(h, p);
+  const bool ring = (direct_a && direct_b) || pack_operands(h, g, p, direct_a, direct_b);
   const Plan16 plan = plan16(p.m, p.n, p.k, g.batch, g.tri != 0, ring, scratch,
                              h->compute_units > 0 ? h->compute_units : 256);
   p.tri = plan.tri;

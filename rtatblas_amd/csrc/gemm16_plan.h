@@ -29,6 +29,24 @@ struct Plan16 {
 // Floats between the columns of a slice's sums.
 inline long slice_ld16(int m) { return ((long)m + 7) / 8 * 8; }
 
+// Whether a product with both operands contiguous along k goes to the kernel for few columns, which
+// cuts k across the waves of a workgroup only: a workgroup reads its sixteen rows at 0.63 us per 1024
+// of k, whatever their number.  Few rows of a long k have too few workgroups to fill memory's pipe; slices
+// of tiles, where there is scratch for them, have 64 times as many.  us, few columns / slices:
+//   rows   k = 16384   20480     24576     32768     65536     1048576
+//     16     13 / 14   15 / 14   18 / 13   23 / 14   44 / 16   682 / 60
+//   1024     14 / 15   17 / 18   19 / 17   24 / 19   45 / 27
+//   2048     16 / 20   17 / 22   20 / 24   25 / 29   49 / 44
+//   4096     25 / 27   27 / 33   30 / 35   39 / 47  103 / 124
+// (one column; where few columns are taken, the slices' time is that of 17).  Sixteen columns take
+// up to 70 % longer here from 2048 x 65536 on, slices of them do not.
+constexpr int FEW_COLS = 16;
+constexpr int FEW_ROWS = 1 << 27;  // 2^23 workgroups of 256: a launch holds fewer than 2^32 threads
+inline bool few_columns16(int m, int n, int k, size_t scratch) {
+  if (n > FEW_COLS || m > FEW_ROWS || k % 8 != 0 || k == 0) return false;
+  return scratch == 0 || m > 2048 || k <= (m <= 1024 ? 20480 : 32768);
+}
+
 inline double price16(int tile, long tiles, long panels, long cus) {
   const long w = (tiles + cus - 1) / cus;  // tiles of the busiest CU
   const double p = (double)panels;

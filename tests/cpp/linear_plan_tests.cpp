@@ -130,3 +130,18 @@ TEST(gemm16_plan, whatever_is_chosen_fits, false) {
                 }
               }
 }
+
+TEST(gemm16_plan, few_columns_of_a_long_k, false) {
+  const size_t scratch = (size_t)64 << 20;
+  CHECK(few_columns16(8192, 1, 2048, scratch) && few_columns16(2048, 13, 8192, scratch) && few_columns16(1, 1, 8, scratch));
+  CHECK(few_columns16(8192, 16, 131072, scratch) && few_columns16(16, 16, 20480, scratch));
+  for (int m : {1, 16, 64, 1000, 1024})
+    for (int k : {24576, 65536, 1 << 20, 1 << 29}) {
+      CHECK(!few_columns16(m, 1, k, scratch) && !few_columns16(m, 16, k, scratch));
+      CHECK(plan16(m, 16, k, 1, false, true, scratch, 256).slices >= 32);
+      CHECK(few_columns16(m, 1, k, 0));  // nothing to cut into
+    }
+  CHECK(!few_columns16(2048, 4, 65536, scratch) && few_columns16(2048, 4, 32768, scratch));
+  CHECK(!few_columns16(64, 17, 64, scratch) && !few_columns16(64, 1, 65, scratch) && !few_columns16(64, 1, 0, scratch));
+  CHECK(!few_columns16((1 << 27) + 1, 1, 8, scratch));
+}
