@@ -428,7 +428,8 @@ rtat_status_t rtat_device_peaks(rtat_handle_t handle, double* fp64_mfma_flops,
  * trsm) launched: the tile shape actually used ("32x32" when the automatic choice took the
  * shape that has no variant id), how many leftover tiles were cut along K and into how many
  * slices, and how many were recomputed as 64 x 64 pieces.  For reports that must name the
- * kernel a figure belongs to.  No counterpart in the reference. */
+ * kernel a figure belongs to.  The products of a linear layer (rtat_gemm_ep and its kin) and
+ * rtat_newton_schulz leave it as it was.  No counterpart in the reference. */
 typedef struct rtat_launch_info {
   char tile[16];       /* "256x128" | "128x128" | "128x64" | "64x64" | "32x32" | "" (no launch) */
   int tiles;           /* tiles of that shape the problem has                                */

@@ -3,7 +3,7 @@
 // Newton-Schulz iteration.  Column-major, D(m x n) = epilogue(op(A) op(B)); f32 accumulation.
 //
 //   * One workgroup computes a BM x BN tile; K advances BK = 64 elements (128 bytes) at a time
-//     through two LDS stages.
+//     through a ring of panels in LDS, or two stages of LDS where operands are not aligned.
 //   * Panels keep the orientation they have in memory.  An operand that is contiguous along k
 //     ("k-major") lies as rows of 64 k, one 16-byte read per lane and MFMA operand; one that is
 //     contiguous along m / n ("mn-major") lies as 64 rows of BM (BN) elements and is read with
@@ -577,8 +577,9 @@ template <int N>
 //   * Smaller tiles run the same schedule, two or four workgroups a CU.  Where so few tiles are
 //     left that one or two a CU are all there is, a ring of eight slots keeps three panels on
 //     their way; a wave is then bound by issuing, and slot numbers modulo a power of two and one
-//     address for several reads leave 104 instructions to a panel instead of 150 (us at 64 x 64,
-//     1024^3: TN 8.0 -> 7.0, NT 11.0 -> 9.5; 128 x 128, 2048 x 2048 x 1024: NT 18.5 -> 15.7).
+//     address for several reads leave 104 instructions to a panel instead of 150 (us, ring of
+//     five / eight: 1024^3 on 64 x 64, TN 7.5 / 6.7, NT 8.7 / 8.2; 2048^3 on 128 x 128, TN
+//     21.2 / 18.5).
 //   * One barrier per panel, half way through it: by then the second half's operands are in
 //     registers, so both slots are free, and of the loads only the last eight may be missing.
 //   * Within a half the LDS reads of the next half and the panel loads are spread behind the
@@ -867,9 +868,10 @@ bool direct(const void* base, long ld, long stride) {
 // Few columns (a single token, or a handful decoded together) of a product whose operands are both
 // contiguous along k: the time is that of reading A once.  A workgroup takes sixteen rows, its
 // waves a share of k each, straight from memory into registers, eight K-steps in flight; the
-// waves' sums meet in LDS.  Sixteen waves read deep enough that 128 workgroups keep memory busy,
-// so nothing is cut across workgroups.  Measured (us; 64 x 64 tiles in slices in brackets):
-// 8192 x 1 x 2048 5.9 (10.9), 2048 x 13 x 8192 9.2 (13.2), 8192 x 16 x 8192 22 (35).
+// waves' sums meet in LDS.  Nothing is cut across workgroups: 128 of them with sixteen waves each
+// read 3.7 TB/s, 512 of them 5.5 to 6.2, and the second launch of a cut costs more than it gives
+// until k is long (few_columns16).  Warm calls in a row, A in the memory-side cache (us; 64 x 64 tiles in slices in
+// brackets): 8192 x 1 x 2048 6.1 (11.2), 2048 x 13 x 8192 9.0 (13.0), 8192 x 16 x 8192 21.5 (25.1).
 constexpr int FEW_DEEP = 8, FEW_WAVES = 16;
 
 template <class T>

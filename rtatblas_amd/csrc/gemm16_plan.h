@@ -9,9 +9,9 @@
 //    64 x 64    3.7 per round of four, and a panel 0.175 per tile of a CU, 0.3 at least
 //   slices      3 for the second launch, and their bytes, written and read once, at 4 MB/us
 //   the mirrored half of a symmetric product: 7 (narrow stores), 3 when slices are joined
-// Examples (us, chosen / the other shapes whole): 4096 x 2048 x 2048 128: 33 / 64: 52, 256: 49;
-// 2048 x 3584 x 4096 128: 61 / 83, 82; 1024^3 64: 6.5 / 128: 11, 256: 25; 768 x 768 x 8192 in
-// slices 23 / 46, 59, 141.
+// Examples (us, chosen / whole tiles of the other shapes): 4096 x 2048 x 2048 128: 33 / 64: 52, 256: 44;
+// 2048 x 3584 x 4096 128: 57 / 64: 85, 256: 78; 1024^3 64: 6.7 / 128: 10, 256: 25; 768 x 768 x 8192 in
+// slices 22 / 64: 28, 128: 45, 256: 144.
 #pragma once
 #include <stddef.h>
 
