@@ -1122,7 +1122,7 @@ __global__ __launch_bounds__(256) void sum_rows_kernel(const float* parts, int c
 
 }  // namespace
 
-int dact_sum_rows(int n) { return 4 * ((n + 63) / 64); }
+int dact_sum_rows(int n) { return (int)(4 * (((long)n + 63) / 64)); }
 
 rtat_status_t launch_sum_rows(rtat_native_handle* h, const float* parts, int count, int m,
                               float* out) {
